@@ -65,7 +65,9 @@ int ms_set_pair_tiles(int enable);
 
 /* Reads and clears the device status word of the current device. Kernels
  * that wait on barriers give up after a bounded time, record a non-zero code
- * there (1 = tensor-core pipeline timeout, 2 = peer timeout) and return.
+ * there (1 = tensor-core pipeline timeout, 2 = peer timeout) and return. The
+ * 4-bit cache's kernels and ms_copy_pages skip a slot, page or length outside
+ * the cache and record 3.
  * Synchronises `stream`. */
 int ms_get_device_status(int* status, void* stream);
 
@@ -190,6 +192,67 @@ int ms_paged_prefill_fp8(const void* q, const void* k_cache, const void* v_cache
  * (microserve/layers/attention.py:49-55). */
 int ms_varlen_prefill(const void* q, const void* k, const void* v, const int32_t* cu, void* out, int num_seqs,
                       int64_t total, int Hq, int Hkv, int head_dim, float softmax_scale, void* stream);
+
+/* ---- 4-bit KV cache (no reference counterpart: its cache is FP8 or fp16) ----
+ *
+ * A (token, kv head) row of head_dim 128 is 64 bytes of e2m1 codes (element 2i in the
+ * low nibble of byte i) and 8 scale bytes, one per 16 elements: unsigned floats of 5
+ * exponent and 3 mantissa bits whose fp16 bits are byte << 7. value = code * scale,
+ * exact in fp16. scale = min(rn(max|x| / 6), 10240), code = rn(x / scale) saturating at
+ * 6, both roundings ties to even; infinities count as 65504; a group of 16 that holds
+ * a NaN is stored with scale byte 0xFF (NaN) and zero codes. 144 bytes per token and
+ * head for K and V, where the FP8 cache takes 264.
+ *   k_cache, v_cache [num_blocks, kv_heads, block_size, 64] uint8
+ *   k_scale, v_scale [num_blocks, kv_heads, block_size, 8] uint8
+ * head_dim == 128, block_size % 64 == 0, num_blocks * block_size < 2^31, all four
+ * 16-byte aligned. Slots, pages and lengths outside the cache are skipped on the GPU
+ * and recorded (device status 3). */
+
+/* Quantise-on-write of k, v [T, kv_heads, 128] fp16 at slots [T] int64 (block *
+ * block_size + offset; negative = skip). Strides in elements (multiples of 8, the
+ * rows 16-byte aligned), so k and v may be slices of a fused projection's output. Two
+ * tokens of a call must not name the same slot. */
+int ms_store_kv_fp4(const void* k, const void* v, int64_t k_token_stride, int64_t k_head_stride,
+                    int64_t v_token_stride, int64_t v_head_stride, int64_t T, int kv_heads, int head_dim,
+                    const int64_t* slots, void* k_cache, void* v_cache, void* k_scale, void* v_scale,
+                    int64_t num_blocks, int block_size, void* stream);
+
+/* The tokens at slots [T] as fp16 rows k, v [T, kv_heads, 128] (exact; zeros for a
+ * negative slot). */
+int ms_load_kv_fp4(const void* k_cache, const void* v_cache, const void* k_scale, const void* v_scale,
+                   int64_t num_blocks, int block_size, int64_t T, int kv_heads, int head_dim, const int64_t* slots,
+                   void* k, void* v, void* stream);
+
+/* ms_paged_decode_fp8 over the 4-bit cache: q [B, Hq, 128] fp16 with a token stride in
+ * elements (heads contiguous), out [B, Hq, 128] fp16 (0 for seqlens == 0). Hq / Hkv <= 8.
+ * A page outside the cache counts as masked, a length above max_blocks * block_size
+ * is cut there (both recorded: device status 3). */
+int ms_paged_decode_fp4(const void* q, int64_t q_token_stride, const void* k_cache, const void* v_cache,
+                        const void* k_scale, const void* v_scale, int64_t num_blocks, const int32_t* seqlens,
+                        const int32_t* block_tables, void* out, int B, int Hq, int Hkv, int head_dim, int block_size,
+                        int max_blocks, float softmax_scale, void* stream);
+
+/* ms_paged_prefill_fp8 over the 4-bit cache, any Hq / Hkv <= 8: sequence s has queries
+ * q[cu_q[s] .. cu_q[s+1]) at positions kv_lens[s] - q_len_s + i, each seeing the keys
+ * up to its own position (none below position 0: output 0). Rows of out behind
+ * cu_q[num_seqs] are not written. */
+int ms_paged_prefill_fp4(const void* q, int64_t q_token_stride, const void* k_cache, const void* v_cache,
+                         const void* k_scale, const void* v_scale, int64_t num_blocks, const int32_t* block_tables,
+                         const int32_t* cu_q, const int32_t* kv_lens, void* out, int num_seqs, int64_t total_q,
+                         int Hq, int Hkv, int head_dim, int block_size, int max_blocks, float softmax_scale,
+                         void* stream);
+
+/* Page copies inside a paged cache (fork of a sequence, moves), all planes (K and V of
+ * every layer), codes and scales in one launch: for i < n, tokens [0, tokens[i]) (null:
+ * whole pages) of page src[i] to page dst[i]. A page is `outer` runs of block_size rows
+ * of row_bytes (scale_row_bytes) each: FP8 cache outer = 1, row_bytes = kv_heads *
+ * head_dim, scale_row_bytes = kv_heads * 4; 4-bit cache outer = kv_heads, 64 and 8. Plane
+ * p's pages start at cache + p * cache_plane_stride bytes. A page may be the source of
+ * any number of pairs but the destination of one, and no page both; pairs outside
+ * [0, num_pages) are skipped (device status 3). No reference counterpart. */
+int ms_copy_pages(void* cache, int64_t cache_plane_stride, int row_bytes, void* scale, int64_t scale_plane_stride,
+                  int scale_row_bytes, int planes, int outer, int block_size, int64_t num_pages, const int32_t* src,
+                  const int32_t* dst, const int32_t* tokens, int n, void* stream);
 
 /* Greedy token selection: idx[m] = argmax_v x[m, v] over fp16 logits rows
  * (row stride ldx elements), the first index of the maximum, NaN above every

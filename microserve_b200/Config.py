@@ -23,8 +23,10 @@
                          shape in model_dir/config.json or `hf_config`);
   hf_config            - a transformers config object used instead of
                          reading model_dir/config.json.
-The FP8 e4m3 KV cache is the only cache this engine implements, so it is the
-default here; fp16 activations are required by the FP8 path (as in the
+kv_cache_dtype: "fp8_e4m3" (the default) or "fp4_e2m1" (4-bit codes with a scale
+per 16 elements: 144 bytes per token, kv head and layer instead of 264, so
+about 1.8 times the tokens fit and attention reads about half); the fp16 cache
+is not implemented. fp16 activations are required by the FP8 path (as in the
 reference).
 """
 import os
@@ -63,9 +65,9 @@ class Config:
         assert self.block_size > 0 and self.block_size % 256 == 0, "block_size must be a multiple of 256"
         assert 0 < self.gpu_memory_utilization <= 1.0
         assert self.quantization in (None, "fp8_dynamic"), "unsupported quantization"
-        assert self.kv_cache_dtype in ("fp16", "fp8_e4m3"), "unsupported KV cache dtype"
-        if self.kv_cache_dtype == "fp8_e4m3":
-            assert self.dtype == torch.float16, "FP8 KV cache currently requires FP16 model dtype"
+        assert self.kv_cache_dtype in ("fp16", "fp8_e4m3", "fp4_e2m1"), "unsupported KV cache dtype"
+        if self.kv_cache_dtype in ("fp8_e4m3", "fp4_e2m1"):
+            assert self.dtype == torch.float16, "FP8 and 4-bit KV caches require FP16 model dtype"
         assert self.scheduler_policy in ("mixed", "prefill_first"), "unsupported scheduler policy"
         assert self.tensor_parallel_size >= 1
         assert self.load_format in ("safetensors", "dummy"), "unsupported load_format"

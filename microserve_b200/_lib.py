@@ -54,6 +54,12 @@ SIGNATURES: dict[str, tuple] = {
     "ms_paged_decode_fp8": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, f32, vp, sz, vp]),
     "ms_paged_decode_fp8_noalloc": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, f32, vp]),
     "ms_paged_prefill_fp8": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, i32, i64, i32, i32, i32, i32, i32, f32, vp]),
+    "ms_store_kv_fp4": (i32, [vp, vp, i64, i64, i64, i64, i64, i32, i32, vp, vp, vp, vp, vp, i64, i32, vp]),
+    "ms_load_kv_fp4": (i32, [vp, vp, vp, vp, i64, i32, i64, i32, i32, vp, vp, vp, vp]),
+    "ms_paged_decode_fp4": (i32, [vp, i64, vp, vp, vp, vp, i64, vp, vp, vp, i32, i32, i32, i32, i32, i32, f32, vp]),
+    "ms_paged_prefill_fp4": (i32, [vp, i64, vp, vp, vp, vp, i64, vp, vp, vp, vp, i32, i64, i32, i32, i32, i32, i32,
+                                   f32, vp]),
+    "ms_copy_pages": (i32, [vp, i64, i32, vp, i64, i32, i32, i32, i32, i64, vp, vp, vp, i32, vp]),
     "ms_varlen_prefill": (i32, [vp, vp, vp, vp, vp, i32, i64, i32, i32, i32, f32, vp]),
 }
 
@@ -103,13 +109,14 @@ def check(rc: int, what: str) -> None:
 
 
 def device_status() -> int:
-    """Read and clear the device status word (non-zero = a bounded wait timed out)."""
+    """Read and clear the device status word (non-zero: see STATUS_NAMES)."""
     s = C.c_int(0)
     check(load().ms_get_device_status(C.byref(s), stream_ptr()), "ms_get_device_status")
     return s.value
 
 
-STATUS_NAMES = {1: "a pipeline barrier wait timed out", 2: "a peer (tensor-parallel rank) did not answer in time"}
+STATUS_NAMES = {1: "a pipeline barrier wait timed out", 2: "a peer (tensor-parallel rank) did not answer in time",
+                3: "a slot, page or length outside the KV cache was skipped"}
 
 
 class DeviceWaitTimeout(RuntimeError):
@@ -118,8 +125,11 @@ class DeviceWaitTimeout(RuntimeError):
 
 
 def raise_on_device_status(where: str) -> None:
-    """Read (and clear) the device status word; raise DeviceWaitTimeout if set."""
+    """Read (and clear) the device status word; if set raise DeviceWaitTimeout (RuntimeError for
+    an address outside the KV cache)."""
     s = device_status()
+    if s == 3:
+        raise RuntimeError(f"{where}: device status 3 ({STATUS_NAMES[3]})")
     if s != 0:
         raise DeviceWaitTimeout(f"{where}: device status {s} ({STATUS_NAMES.get(s, 'unknown')})")
 

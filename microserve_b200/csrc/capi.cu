@@ -48,6 +48,36 @@ int num_sms() {
 
 inline cudaStream_t S(void* s) { return reinterpret_cast<cudaStream_t>(s); }
 
+inline bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+// The 4-bit cache's own limits, shared by its entry points.
+int check_fp4_cache(const char* what, const void* k_cache, const void* v_cache, const void* k_scale,
+                    const void* v_scale, int64_t num_blocks, int kv_heads, int head_dim, int block_size) {
+  if (kv_heads <= 0 || num_blocks <= 0 || block_size <= 0) return fail(MS_ERR_INVALID, "%s: bad sizes", what);
+  if (head_dim != 128) return fail(MS_ERR_UNSUPPORTED, "%s: head_dim %d != 128", what, head_dim);
+  if (block_size % 64 != 0)
+    return fail(MS_ERR_UNSUPPORTED, "%s: block_size %d is not a multiple of 64", what, block_size);
+  if (num_blocks > INT32_MAX / block_size)
+    return fail(MS_ERR_UNSUPPORTED, "%s: %lld blocks of %d tokens exceed 2^31 - 1 slots", what, (long long)num_blocks,
+                block_size);
+  if (!k_cache || !v_cache || !k_scale || !v_scale) return fail(MS_ERR_INVALID, "%s: null cache pointer", what);
+  if (!aligned16(k_cache) || !aligned16(v_cache) || !aligned16(k_scale) || !aligned16(v_scale))
+    return fail(MS_ERR_INVALID, "%s: caches must be 16-byte aligned", what);
+  return MS_OK;
+}
+
+// Query / output layout of the attentions over the 4-bit cache.
+int check_fp4_query(const char* what, const void* q, int64_t q_stride, const void* out, int Hq, int Hkv) {
+  if (Hq <= 0 || Hq % Hkv != 0 || Hq / Hkv > 8)
+    return fail(MS_ERR_UNSUPPORTED, "%s: Hq=%d Hkv=%d unsupported (Hq a multiple of Hkv, at most 8 per kv head)", what,
+                Hq, Hkv);
+  if (!q || !out) return fail(MS_ERR_INVALID, "%s: null pointer", what);
+  if (!aligned16(q) || !aligned16(out) || q_stride < (int64_t)Hq * 128 || q_stride % 8 != 0)
+    return fail(MS_ERR_INVALID, "%s: q and out must be 16-byte aligned, q's token stride a multiple of 8 elements",
+                what);
+  return MS_OK;
+}
+
 }  // namespace
 
 extern "C" {
@@ -275,6 +305,104 @@ int ms_varlen_prefill(const void* q, const void* k, const void* v, const int32_t
                                                  nullptr, out, num_seqs, (int)total, Hq, Hkv, head_dim, 256, 1,
                                                  softmax_scale, S(stream)),
                     "ms_varlen_prefill");
+}
+
+// --------------------------------------------------------------------------- 4-bit KV cache
+int ms_store_kv_fp4(const void* k, const void* v, int64_t k_token_stride, int64_t k_head_stride,
+                    int64_t v_token_stride, int64_t v_head_stride, int64_t T, int kv_heads, int head_dim,
+                    const int64_t* slots, void* k_cache, void* v_cache, void* k_scale, void* v_scale,
+                    int64_t num_blocks, int block_size, void* stream) {
+  if (T < 0 || T > INT32_MAX) return fail(MS_ERR_INVALID, "ms_store_kv_fp4: bad sizes T=%lld", (long long)T);
+  const int rc = check_fp4_cache("ms_store_kv_fp4", k_cache, v_cache, k_scale, v_scale, num_blocks, kv_heads,
+                                 head_dim, block_size);
+  if (rc != MS_OK || T == 0) return rc;
+  if (!k || !v || !slots) return fail(MS_ERR_INVALID, "ms_store_kv_fp4: null pointer");
+  const int64_t st[4] = {k_token_stride, k_head_stride, v_token_stride, v_head_stride};
+  for (int64_t x : st)
+    if (x < 0 || x % 8 != 0) return fail(MS_ERR_INVALID, "ms_store_kv_fp4: strides must be multiples of 8 elements");
+  if (!aligned16(k) || !aligned16(v)) return fail(MS_ERR_INVALID, "ms_store_kv_fp4: k and v must be 16-byte aligned");
+  return check_cuda(ms::launch_store_kv_fp4(k, v, k_token_stride, k_head_stride, v_token_stride, v_head_stride, T,
+                                            kv_heads, slots, k_cache, v_cache, k_scale, v_scale, num_blocks,
+                                            block_size, S(stream)),
+                    "ms_store_kv_fp4");
+}
+
+int ms_load_kv_fp4(const void* k_cache, const void* v_cache, const void* k_scale, const void* v_scale,
+                   int64_t num_blocks, int block_size, int64_t T, int kv_heads, int head_dim, const int64_t* slots,
+                   void* k, void* v, void* stream) {
+  if (T < 0 || T > INT32_MAX) return fail(MS_ERR_INVALID, "ms_load_kv_fp4: bad sizes T=%lld", (long long)T);
+  const int rc = check_fp4_cache("ms_load_kv_fp4", k_cache, v_cache, k_scale, v_scale, num_blocks, kv_heads, head_dim,
+                                 block_size);
+  if (rc != MS_OK || T == 0) return rc;
+  if (!k || !v || !slots) return fail(MS_ERR_INVALID, "ms_load_kv_fp4: null pointer");
+  if (!aligned16(k) || !aligned16(v)) return fail(MS_ERR_INVALID, "ms_load_kv_fp4: k and v must be 16-byte aligned");
+  return check_cuda(ms::launch_load_kv_fp4(k_cache, v_cache, k_scale, v_scale, num_blocks, block_size, T, kv_heads,
+                                           slots, k, v, S(stream)),
+                    "ms_load_kv_fp4");
+}
+
+int ms_paged_decode_fp4(const void* q, int64_t q_token_stride, const void* k_cache, const void* v_cache,
+                        const void* k_scale, const void* v_scale, int64_t num_blocks, const int32_t* seqlens,
+                        const int32_t* block_tables, void* out, int B, int Hq, int Hkv, int head_dim, int block_size,
+                        int max_blocks, float softmax_scale, void* stream) {
+  if (B < 0 || max_blocks <= 0) return fail(MS_ERR_INVALID, "ms_paged_decode_fp4: bad sizes");
+  int rc = check_fp4_cache("ms_paged_decode_fp4", k_cache, v_cache, k_scale, v_scale, num_blocks, Hkv, head_dim,
+                           block_size);
+  if (rc != MS_OK) return rc;
+  if (B == 0) return MS_OK;
+  rc = check_fp4_query("ms_paged_decode_fp4", q, q_token_stride, out, Hq, Hkv);
+  if (rc != MS_OK) return rc;
+  if (!seqlens || !block_tables) return fail(MS_ERR_INVALID, "ms_paged_decode_fp4: null pointer");
+  return check_cuda(ms::launch_fp4_attention(q, q_token_stride, k_cache, v_cache, k_scale, v_scale, num_blocks,
+                                             block_tables, nullptr, seqlens, out, B, B, Hq, Hkv, block_size,
+                                             max_blocks, softmax_scale, S(stream)),
+                    "ms_paged_decode_fp4");
+}
+
+int ms_paged_prefill_fp4(const void* q, int64_t q_token_stride, const void* k_cache, const void* v_cache,
+                         const void* k_scale, const void* v_scale, int64_t num_blocks, const int32_t* block_tables,
+                         const int32_t* cu_q, const int32_t* kv_lens, void* out, int num_seqs, int64_t total_q,
+                         int Hq, int Hkv, int head_dim, int block_size, int max_blocks, float softmax_scale,
+                         void* stream) {
+  if (num_seqs < 0 || total_q < 0 || max_blocks <= 0 || total_q > INT32_MAX)
+    return fail(MS_ERR_INVALID, "ms_paged_prefill_fp4: bad sizes");
+  int rc = check_fp4_cache("ms_paged_prefill_fp4", k_cache, v_cache, k_scale, v_scale, num_blocks, Hkv, head_dim,
+                           block_size);
+  if (rc != MS_OK) return rc;
+  if (num_seqs == 0 || total_q == 0) return MS_OK;
+  rc = check_fp4_query("ms_paged_prefill_fp4", q, q_token_stride, out, Hq, Hkv);
+  if (rc != MS_OK) return rc;
+  if (!block_tables || !cu_q || !kv_lens) return fail(MS_ERR_INVALID, "ms_paged_prefill_fp4: null pointer");
+  return check_cuda(ms::launch_fp4_attention(q, q_token_stride, k_cache, v_cache, k_scale, v_scale, num_blocks,
+                                             block_tables, cu_q, kv_lens, out, num_seqs, (int)total_q, Hq, Hkv,
+                                             block_size, max_blocks, softmax_scale, S(stream)),
+                    "ms_paged_prefill_fp4");
+}
+
+int ms_copy_pages(void* cache, int64_t cache_plane_stride, int row_bytes, void* scale, int64_t scale_plane_stride,
+                  int scale_row_bytes, int planes, int outer, int block_size, int64_t num_pages, const int32_t* src,
+                  const int32_t* dst, const int32_t* tokens, int n, void* stream) {
+  if (n < 0 || planes < 0 || outer <= 0 || block_size <= 0 || num_pages <= 0 || num_pages > INT32_MAX ||
+      row_bytes <= 0 || scale_row_bytes <= 0)
+    return fail(MS_ERR_INVALID, "ms_copy_pages: bad sizes");
+  if (n == 0 || planes == 0) return MS_OK;
+  if (!cache || !scale || !src || !dst) return fail(MS_ERR_INVALID, "ms_copy_pages: null pointer");
+  const int rows[2] = {row_bytes, scale_row_bytes};
+  const int64_t strides[2] = {cache_plane_stride, scale_plane_stride};
+  const void* base[2] = {cache, scale};
+  for (int i = 0; i < 2; ++i) {
+    const int64_t run = (int64_t)block_size * rows[i];
+    if (rows[i] % 4 != 0 || run % 16 != 0 || run > (1 << 30))
+      return fail(MS_ERR_UNSUPPORTED, "ms_copy_pages: %d rows of %d bytes are not 16-byte vectors", block_size,
+                  rows[i]);
+    if (strides[i] % 16 != 0 || (planes > 1 && strides[i] < run * outer * num_pages))
+      return fail(MS_ERR_INVALID, "ms_copy_pages: bad plane stride %lld", (long long)strides[i]);
+    if (!aligned16(base[i])) return fail(MS_ERR_INVALID, "ms_copy_pages: caches must be 16-byte aligned");
+  }
+  return check_cuda(ms::launch_copy_pages(cache, cache_plane_stride, row_bytes, scale, scale_plane_stride,
+                                          scale_row_bytes, planes, outer, block_size, num_pages, src, dst, tokens, n,
+                                          num_sms(), S(stream)),
+                    "ms_copy_pages");
 }
 
 size_t ms_argmax_workspace_size(int64_t M) { return M > 0 ? ms::argmax_workspace_bytes(M) : 0; }

@@ -34,6 +34,7 @@ enum DeviceStatus : int {
   kStatusOk = 0,
   kStatusMbarTimeout = 1,
   kStatusPeerTimeout = 2,
+  kStatusBadPage = 3,  // a slot, page or length outside the cache was skipped (4-bit cache, page copies)
 };
 
 extern __device__ int g_device_status;

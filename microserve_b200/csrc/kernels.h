@@ -41,6 +41,26 @@ cudaError_t launch_prefill_attention(bool paged, const void* q, const void* k16,
                                      int head_dim, int block_size, int max_blocks, float softmax_scale,
                                      cudaStream_t stream);
 
+// 4-bit KV cache (fp4_kv.cuh). Strides in elements; caches as uint8 codes and scales.
+cudaError_t launch_store_kv_fp4(const void* k, const void* v, int64_t k_ts, int64_t k_hs, int64_t v_ts, int64_t v_hs,
+                                int64_t T, int kv_heads, const int64_t* slots, void* k_cache, void* v_cache,
+                                void* k_scale, void* v_scale, int64_t num_blocks, int block_size,
+                                cudaStream_t stream);
+cudaError_t launch_load_kv_fp4(const void* k_cache, const void* v_cache, const void* k_scale, const void* v_scale,
+                               int64_t num_blocks, int block_size, int64_t T, int kv_heads, const int64_t* slots,
+                               void* k, void* v, cudaStream_t stream);
+// cu_q null: decode (one query per sequence)
+cudaError_t launch_fp4_attention(const void* q, int64_t q_ts, const void* k_cache, const void* v_cache,
+                                 const void* k_scale, const void* v_scale, int64_t num_blocks,
+                                 const int32_t* block_tables, const int32_t* cu_q, const int32_t* kv_lens, void* out,
+                                 int num_seqs, int total_q, int Hq, int Hkv, int block_size, int max_blocks,
+                                 float softmax_scale, cudaStream_t stream);
+
+cudaError_t launch_copy_pages(void* cache, int64_t cache_plane_stride, int row_bytes, void* scale,
+                              int64_t scale_plane_stride, int scale_row_bytes, int planes, int outer, int block_size,
+                              int64_t num_pages, const int32_t* src, const int32_t* dst, const int32_t* tokens, int n,
+                              int num_sms, cudaStream_t stream);
+
 // One rank's communication buffer for the fused tensor-parallel op: byte offsets
 // (peers write [recv, ctrl); outq/outs/outh are the normalised rows this rank's
 // next op reads).

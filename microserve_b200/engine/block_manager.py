@@ -133,6 +133,23 @@ class BlockManager:
             seq.block_table.append(self._take_free())
         return True
 
+    def fork(self, parent: Sequence, child: Sequence) -> list[tuple[int, int, int]]:
+        """Give `child` (a copy of `parent` at its computed tokens, without blocks) a block table: the full
+        blocks are shared (one more reference each: nothing writes to a full block again), the partly
+        filled last one gets a block of its own. Returns the (src, dst, tokens) page copies still to be
+        made. Raises RuntimeError, with nothing changed, if that block is not to be had."""
+        full, rest = divmod(parent.num_computed_tokens, self.block_size)
+        if rest and not self.free_blocks:
+            raise RuntimeError("fork: no free KV block for the partly filled last page")
+        for bid in parent.block_table[:full]:
+            self.blocks[bid].ref_count += 1
+        child.block_table = parent.block_table[:full]
+        if not rest:
+            return []
+        bid = self._take_free()
+        child.block_table.append(bid)
+        return [(parent.block_table[full], bid, rest)]
+
     def deallocate(self, seq: Sequence) -> None:
         for bid in reversed(seq.block_table):
             self._unref(bid)

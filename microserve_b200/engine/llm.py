@@ -1,7 +1,7 @@
 """Serving front end: one model runner (weights, KV cache, CUDA graphs) driven by
 one scheduler. Public surface as the reference's LLMEngine
 (microserve/engine/llm.py:6-53): LLMEngine(config), add(), step(), is_idle(),
-generate(), num_running().
+generate(), num_running(); plus fork().
 
 A step is: ask the scheduler for a batch, run it on the GPU (the runner checks
 the device status word after every step, so a bounded in-kernel wait that ran
@@ -31,6 +31,22 @@ class LLMEngine:
         seq = Sequence(token_ids, sampling_params=sampling_params, max_tokens=max_tokens)
         self.scheduler.add(seq)
         return seq
+
+    def fork(self, seq: Sequence, sampling_params: SamplingParams | None = None,
+             max_tokens: int | None = None) -> Sequence:
+        """A second sequence that continues from `seq`'s tokens and KV cache, between two steps (several
+        samples of one prompt, a branch of a search). Full KV pages are shared; the partly filled
+        last one is copied. The fork counts seq's prompt as its own and seq's completion so far as its
+        completion; its sampling parameters and max_tokens default to seq's. Raises ValueError if seq
+        is not running or max_tokens is already reached, RuntimeError if max_num_seqs or the free KV
+        blocks do not allow it."""
+        child = Sequence(seq.token_ids, sampling_params=sampling_params or seq.sampling_params,
+                         max_tokens=seq.max_tokens if max_tokens is None else max_tokens)
+        child.num_prompt_tokens = seq.num_prompt_tokens
+        copies = self.scheduler.fork(seq, child)
+        if copies:
+            self.runner.copy_pages(copies)
+        return child
 
     def step(self) -> list[Sequence]:
         """Schedule and execute one batch; the sequences that finished in it."""

@@ -1,4 +1,4 @@
-"""Model runner: weights, FP8 KV cache, batch preparation, decode CUDA graphs
+"""Model runner: weights, FP8 or 4-bit KV cache, batch preparation, decode CUDA graphs
 and sampling (microserve/engine/model_runner.py:36-338), B200 version.
 
 Same responsibilities and the same integer formulas as the reference:
@@ -26,6 +26,7 @@ from microserve_b200.Config import Config
 from microserve_b200 import _lib, kernels
 from microserve_b200.engine.sequence import Sequence
 from microserve_b200.layers.attention import Attention
+from microserve_b200.layers.fp4_kv_cache import allocate_fp4_kvcache
 from microserve_b200.layers.fp8_linear import quantize_fp8_linears
 from microserve_b200.models.qwen3 import Qwen3ForCausalLM
 from microserve_b200.utils import dist as tp
@@ -125,7 +126,7 @@ class ModelRunner:
         # FP8 quantisation that follow them, over peer memory (utils/tp_fused.py).
         self.tp_fused = None
         if (tp.tp_size() > 1 and config.tp_fused_collective and self.num_quantized_linears > 0
-                and config.kv_cache_dtype == "fp8_e4m3"):
+                and config.kv_cache_dtype in ("fp8_e4m3", "fp4_e2m1")):
             from microserve_b200.utils.tp_fused import TpFused
             rows = max(config.max_num_batched_tokens, (config.max_num_seqs + 15) // 16 * 16)
             self.tp_fused = TpFused(rows, hf.hidden_size, self.device, fused_gemm=config.tp_fused_gemm)
@@ -135,10 +136,15 @@ class ModelRunner:
         if self.num_blocks <= 0:
             self.num_blocks = self._auto_num_blocks()
         self.garbage_slot = self.num_blocks * self.block_size
-        cache_dtype = torch.float8_e4m3fn if config.kv_cache_dtype == "fp8_e4m3" else config.dtype
-        self.kv_cache = torch.zeros(2, self.num_layers, self.num_blocks + 1, self.block_size, self.num_kv_heads,
-                                    self.head_dim, dtype=cache_dtype, device=self.device)
         self.kv_scale_cache = None
+        if config.kv_cache_dtype == "fp4_e2m1":
+            self.kv_cache, self.kv_scale_cache = allocate_fp4_kvcache(
+                self.num_blocks + 1, self.block_size, self.num_kv_heads, self.head_dim, self.device,
+                lead=(2, self.num_layers))
+        else:
+            cache_dtype = torch.float8_e4m3fn if config.kv_cache_dtype == "fp8_e4m3" else config.dtype
+            self.kv_cache = torch.zeros(2, self.num_layers, self.num_blocks + 1, self.block_size, self.num_kv_heads,
+                                        self.head_dim, dtype=cache_dtype, device=self.device)
         if config.kv_cache_dtype == "fp8_e4m3":
             self.kv_scale_cache = torch.ones(2, self.num_layers, self.num_blocks + 1, self.block_size,
                                              self.num_kv_heads, dtype=torch.float32, device=self.device)
@@ -160,6 +166,9 @@ class ModelRunner:
         free, total = torch.cuda.mem_get_info()
         if cfg.kv_cache_dtype == "fp8_e4m3":
             per_block = 2 * self.num_layers * self.block_size * self.num_kv_heads * (self.head_dim + 4)
+        elif cfg.kv_cache_dtype == "fp4_e2m1":
+            per_block = 2 * self.num_layers * self.block_size * self.num_kv_heads * (self.head_dim // 2 +
+                                                                                     self.head_dim // 16)
         else:
             per_block = 2 * self.num_layers * self.block_size * self.num_kv_heads * self.head_dim * 2
         available = (free + total * (cfg.gpu_memory_utilization - 1.0)) * 0.8
@@ -177,6 +186,14 @@ class ModelRunner:
                 module.kv_cache_dtype = self.config.kv_cache_dtype
                 layer_id += 1
         assert layer_id == self.num_layers
+
+    def copy_pages(self, pairs: list[tuple[int, int, int]]) -> None:
+        """Copy the first `tokens` tokens of page `src` to page `dst` in every layer's K and V, for each
+        (src, dst, tokens) (one launch, ordered with the steps on this stream)."""
+        if self.kv_scale_cache is None:
+            raise NotImplementedError("page copies need the FP8 or the 4-bit KV cache")
+        src, dst, tokens = self.host_batch.upload([np.asarray(c, dtype=np.int32) for c in zip(*pairs)])
+        kernels.copy_pages(self.kv_cache, self.kv_scale_cache, src, dst, tokens)
 
     # ------------------------------------------------------- batch preparation
     def _slots(self, table: list[int], positions: np.ndarray) -> np.ndarray:

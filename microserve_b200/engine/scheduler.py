@@ -76,6 +76,23 @@ class Scheduler:
         seq.waiting_entered_at = now
         self.waiting.append(seq)
 
+    def fork(self, parent: Sequence, child: Sequence) -> list[tuple[int, int, int]]:
+        """Admit `child`, a copy of the running `parent`, as a running sequence that continues from
+        the parent's computed tokens (no counterpart in the reference). Between steps only.
+        Returns the page copies to make before the next step (BlockManager.fork)."""
+        if parent not in self.running or parent.num_computed_tokens == 0:
+            raise ValueError("fork: the sequence is not running (queued, finished or preempted)")
+        if child.num_completion_tokens >= child.max_tokens:
+            raise ValueError(f"fork: max_tokens={child.max_tokens} is already reached")
+        if len(self.running) >= self.max_num_seqs:
+            raise RuntimeError(f"fork: {len(self.running)} sequences are running already (max_num_seqs)")
+        copies = self.block_manager.fork(parent, child)
+        child.num_computed_tokens = parent.num_computed_tokens
+        child.status = SequenceStatus.RUNNING
+        child.arrived_at = child.waiting_entered_at = child.first_scheduled_at = perf_counter()
+        self.running.append(child)
+        return copies
+
     def is_idle(self) -> bool:
         return len(self.waiting) == 0 and len(self.running) == 0
 

@@ -305,3 +305,186 @@ def argmax_rows(x: torch.Tensor, want_max: bool = False):
     check(lib.ms_argmax_rows(ptr(x), M, V, x.stride(0), ptr(idx), ptr(vmax), ptr(ws),
                              0 if ws is None else ws.numel(), stream_ptr()), "ms_argmax_rows")
     return (idx, vmax) if want_max else idx
+
+
+# ------------------------------------------------------------------ 4-bit KV cache
+def fp4_cache_shapes(num_blocks: int, block_size: int, kv_heads: int, head_dim: int = 128):
+    """Shapes (codes, scales) of one of the two halves (keys or values) of a 4-bit cache; both uint8."""
+    return (num_blocks, kv_heads, block_size, head_dim // 2), (num_blocks, kv_heads, block_size, head_dim // 16)
+
+
+def _on_current_device(what: str, *tensors: torch.Tensor) -> None:
+    """Every tensor on the current CUDA device, whose current stream the kernel runs on."""
+    dev = torch.cuda.current_device() if tensors[0].is_cuda else -1
+    for t in tensors:
+        if t.get_device() != dev or dev < 0:
+            raise ValueError(f"{what}: every tensor must be on the current CUDA device (one is on {t.device}; "
+                             "use torch.cuda.device(...))")
+
+
+def _fp4_cache(what: str, k_cache, v_cache, k_scale, v_scale, head_dim: int) -> tuple[int, int, int]:
+    """Checks the four tensors of a 4-bit cache; (num_blocks, kv_heads, block_size)."""
+    NB, Hkv, BS, half = shape = k_cache.shape
+    if half * 2 != head_dim:
+        raise ValueError(f"{what}: head_dim {head_dim} does not match a cache of {half} code bytes a row")
+    if v_cache.shape != shape or k_scale.shape != v_scale.shape or k_scale.shape != (NB, Hkv, BS, half // 8):
+        raise ValueError(f"{what}: cache shapes {tuple(shape)} {tuple(v_cache.shape)} {tuple(k_scale.shape)} "
+                         f"{tuple(v_scale.shape)} do not belong together")
+    for t in (k_cache, v_cache, k_scale, v_scale):
+        if t.dtype is not torch.uint8 or not t.is_contiguous():
+            raise ValueError(f"{what}: the 4-bit cache is contiguous uint8")
+    return NB, Hkv, BS
+
+
+def _vector_rows(t: torch.Tensor) -> tuple[torch.Tensor, int, int]:
+    """(t, token stride, head stride) of t [T, heads, 128], itself where a kernel can read its rows as
+    16-byte vectors, else a contiguous copy (of a tensor at an address that is not, a clone)."""
+    ts, hs, one = t.stride()
+    if one == 1 and ts % 8 == 0 and hs % 8 == 0 and t.data_ptr() % 16 == 0:
+        return t, ts, hs
+    t = t.contiguous() if t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
+    return t, t.shape[1] * t.shape[2], t.shape[2]
+
+
+def store_kv_fp4(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                 k_scale: torch.Tensor, v_scale: torch.Tensor, slot_mapping: torch.Tensor) -> None:
+    """Quantise key / value [T, Hkv, 128] fp16 (any token and head stride) into the 4-bit cache at
+    slot_mapping [T] int64 (negative: skipped; no slot twice). ms_store_kv_fp4."""
+    T, Hkv, D = key.shape
+    NB, H, BS = _fp4_cache("store_kv_fp4", k_cache, v_cache, k_scale, v_scale, D)
+    if value.shape != key.shape or H != Hkv or key.dtype is not torch.float16 or value.dtype is not torch.float16:
+        raise ValueError("store_kv_fp4: key and value must be fp16 [T, kv_heads, head_dim] of the cache's heads")
+    if slot_mapping.dtype is not torch.int64 or slot_mapping.shape != (T,) or not slot_mapping.is_contiguous():
+        raise ValueError("store_kv_fp4: slot_mapping must be contiguous int64 [T]")
+    _on_current_device("store_kv_fp4", key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping)
+    key, kts, khs = _vector_rows(key)
+    value, vts, vhs = _vector_rows(value)
+    check(_lib.load().ms_store_kv_fp4(key.data_ptr(), value.data_ptr(), kts, khs, vts, vhs, T, Hkv, D,
+                                      slot_mapping.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(),
+                                      k_scale.data_ptr(), v_scale.data_ptr(), NB, BS, stream_ptr()),
+          "ms_store_kv_fp4")
+
+
+def load_kv_fp4(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                slot_mapping: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """The tokens at slot_mapping [T] int64 of the 4-bit cache as fp16 (k, v) [T, Hkv, 128], exactly
+    the stored values (zeros for negative slots). ms_load_kv_fp4."""
+    NB, Hkv, BS = _fp4_cache("load_kv_fp4", k_cache, v_cache, k_scale, v_scale, 128)
+    if slot_mapping.dtype is not torch.int64 or slot_mapping.dim() != 1 or not slot_mapping.is_contiguous():
+        raise ValueError("load_kv_fp4: slot_mapping must be contiguous int64 [T]")
+    _on_current_device("load_kv_fp4", k_cache, v_cache, k_scale, v_scale, slot_mapping)
+    T = slot_mapping.shape[0]
+    k = torch.empty((T, Hkv, 128), dtype=torch.float16, device=k_cache.device)
+    v = torch.empty_like(k)
+    check(_lib.load().ms_load_kv_fp4(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
+                                     NB, BS, T, Hkv, 128, slot_mapping.data_ptr(), k.data_ptr(), v.data_ptr(),
+                                     stream_ptr()), "ms_load_kv_fp4")
+    return k, v
+
+
+def _fp4_query(what: str, query: torch.Tensor,
+               out: torch.Tensor | None) -> tuple[torch.Tensor, int, torch.Tensor]:
+    """(query whose heads a kernel can read in place, its token stride, the output tensor)."""
+    if query.dtype is not torch.float16 or query.dim() != 3:
+        raise ValueError(f"{what}: query must be fp16 [tokens, heads, head_dim]")
+    if out is None:
+        out = torch.empty(query.shape, dtype=torch.float16, device=query.device)
+    elif out.shape != query.shape or out.dtype is not torch.float16 or not out.is_contiguous():
+        raise ValueError(f"{what}: out must be contiguous fp16 of query's shape")
+    elif out.data_ptr() % 16 != 0:
+        raise ValueError(f"{what}: out must be 16-byte aligned")
+    query, ts, hs = _vector_rows(query)
+    row = query.shape[1] * query.shape[2]
+    if ts < row or hs != query.shape[2]:  # overlapping or interleaved heads, or a single token
+        query, ts = query.contiguous(), row
+    return query, ts, out
+
+
+def _int32(what: str, name: str, t: torch.Tensor, *shape: int) -> None:
+    if t.dtype is not torch.int32 or not t.is_contiguous() or t.dim() != len(shape) \
+            or any(s >= 0 and s != n for s, n in zip(shape, t.shape)):
+        raise ValueError(f"{what}: {name} must be contiguous int32 of shape "
+                         f"[{', '.join('*' if s < 0 else str(s) for s in shape)}]")
+
+
+def paged_decode_fp4(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                     v_scale: torch.Tensor, cache_seqlens: torch.Tensor, block_tables: torch.Tensor,
+                     softmax_scale: float, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Decode attention of query [B, Hq, 128] fp16 (any token stride) over each sequence's first
+    cache_seqlens[b] tokens of the 4-bit cache; 0 for an empty sequence. ms_paged_decode_fp4."""
+    B, Hq, D = query.shape
+    NB, Hkv, BS = _fp4_cache("paged_decode_fp4", k_cache, v_cache, k_scale, v_scale, D)
+    _int32("paged_decode_fp4", "cache_seqlens", cache_seqlens, B)
+    _int32("paged_decode_fp4", "block_tables", block_tables, B, -1)
+    query, q_stride, o = _fp4_query("paged_decode_fp4", query, out)
+    _on_current_device("paged_decode_fp4", query, k_cache, v_cache, k_scale, v_scale, cache_seqlens, block_tables, o)
+    check(_lib.load().ms_paged_decode_fp4(query.data_ptr(), q_stride, k_cache.data_ptr(), v_cache.data_ptr(),
+                                          k_scale.data_ptr(), v_scale.data_ptr(), NB, cache_seqlens.data_ptr(),
+                                          block_tables.data_ptr(), o.data_ptr(), B, Hq, Hkv, D, BS,
+                                          block_tables.shape[1], float(softmax_scale), stream_ptr()),
+          "ms_paged_decode_fp4")
+    return o
+
+
+def paged_prefill_fp4(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                      v_scale: torch.Tensor, block_tables: torch.Tensor, cu_q: torch.Tensor, kv_lens: torch.Tensor,
+                      softmax_scale: float, out: torch.Tensor | None = None) -> torch.Tensor:
+    """Causal attention of new tokens query [T, Hq, 128] fp16 (any token stride) over prefix + themselves
+    in the 4-bit cache, every sequence in one launch. Rows behind cu_q[-1] are not written (pass `out`
+    to keep theirs). ms_paged_prefill_fp4."""
+    T, Hq, D = query.shape
+    NB, Hkv, BS = _fp4_cache("paged_prefill_fp4", k_cache, v_cache, k_scale, v_scale, D)
+    num_seqs = kv_lens.shape[0]
+    _int32("paged_prefill_fp4", "kv_lens", kv_lens, num_seqs)
+    _int32("paged_prefill_fp4", "cu_q", cu_q, num_seqs + 1)
+    _int32("paged_prefill_fp4", "block_tables", block_tables, num_seqs, -1)
+    query, q_stride, o = _fp4_query("paged_prefill_fp4", query, out)
+    _on_current_device("paged_prefill_fp4", query, k_cache, v_cache, k_scale, v_scale, block_tables, cu_q, kv_lens, o)
+    check(_lib.load().ms_paged_prefill_fp4(query.data_ptr(), q_stride, k_cache.data_ptr(), v_cache.data_ptr(),
+                                           k_scale.data_ptr(), v_scale.data_ptr(), NB, block_tables.data_ptr(),
+                                           cu_q.data_ptr(), kv_lens.data_ptr(), o.data_ptr(), num_seqs, T, Hq, Hkv,
+                                           D, BS, block_tables.shape[1], float(softmax_scale), stream_ptr()),
+          "ms_paged_prefill_fp4")
+    return o
+
+
+# ------------------------------------------------------------------ page copies
+def copy_pages(cache: torch.Tensor, scale: torch.Tensor, src: torch.Tensor, dst: torch.Tensor,
+               num_tokens: torch.Tensor | None = None) -> None:
+    """Copy tokens [0, num_tokens[i]) (None: whole pages) of page src[i] to page dst[i] in every plane of
+    a paged cache, codes and scales in one launch. ms_copy_pages.
+
+    cache / scale: the FP8 cache [..., NB, BS, Hkv, D] e4m3 with [..., NB, BS, Hkv] fp32, or the 4-bit one
+    [..., NB, Hkv, BS, 64] with [..., NB, Hkv, BS, 8] uint8; the leading dimensions (layers, K and V) are
+    planes. src, dst, num_tokens: int32 [n] on the GPU. No page may be a destination twice, or both a
+    source and a destination (the pairs run in any order)."""
+    fp8 = cache.dtype is FP8
+    if not fp8 and cache.dtype is not torch.uint8 or cache.dim() < 4:
+        raise ValueError("copy_pages: expected an FP8 cache [..., pages, page_size, heads, dim] or a 4-bit one")
+    lead, (NB, a, b, row) = cache.shape[:-4], cache.shape[-4:]
+    if fp8:
+        ok = scale.dtype is torch.float32 and scale.shape == cache.shape[:-1]
+        outer, BS, row, srow = 1, a, b * row, b * 4
+    else:
+        ok = scale.dtype is torch.uint8 and scale.shape == (*cache.shape[:-1], row // 8)
+        outer, BS, srow = a, b, row // 8
+    if not ok:
+        raise ValueError(f"copy_pages: scales {scale.dtype} {tuple(scale.shape)} do not belong to a cache "
+                         f"{cache.dtype} {tuple(cache.shape)}")
+    if not cache.is_contiguous() or not scale.is_contiguous():
+        raise ValueError("copy_pages: caches must be contiguous")
+    n = src.shape[0]
+    _int32("copy_pages", "src", src, n)
+    _int32("copy_pages", "dst", dst, n)
+    if num_tokens is not None:
+        _int32("copy_pages", "num_tokens", num_tokens, n)
+        _on_current_device("copy_pages", cache, scale, src, dst, num_tokens)
+    else:
+        _on_current_device("copy_pages", cache, scale, src, dst)
+    planes = 1
+    for d in lead:
+        planes *= d
+    pages = NB * outer * BS
+    check(_lib.load().ms_copy_pages(cache.data_ptr(), pages * row, row, scale.data_ptr(), pages * srow, srow, planes,
+                                    outer, BS, NB, src.data_ptr(), dst.data_ptr(), ptr(num_tokens), n, stream_ptr()),
+          "ms_copy_pages")

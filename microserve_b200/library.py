@@ -21,6 +21,9 @@ compose with torch, e.g. the reference's layers replaced op by op:
     layers/fp8_chunk_prefill_attention.py:77-109         paged_prefill_fp8
     layers/attention.py:49-55   flash_attn_varlen_func   varlen_prefill
     engine/model_runner.py:33-34 greedy torch.argmax     argmax_rows
+
+Without a call site in the reference: the 4-bit KV cache (store_kv_fp4, load_kv_fp4,
+paged_decode_fp4, paged_prefill_fp4) and page copies inside a paged cache (copy_pages).
 """
 from __future__ import annotations
 
@@ -235,6 +238,72 @@ def _(q, k, v, cu_seqlens, softmax_scale):
     return torch.empty_like(q)
 
 
+# ------------------------------------------------------------------ 4-bit KV cache, page copies
+@custom_op(f"{_NS}::store_kv_fp4", mutates_args=_CACHES)
+def store_kv_fp4(key: torch.Tensor, value: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+                 k_scale: torch.Tensor, v_scale: torch.Tensor, slot_mapping: torch.Tensor) -> None:
+    """key/value [T, Hkv, 128] fp16 -> e2m1 codes and one scale per 16 elements, scattered to slot_mapping."""
+    kernels.store_kv_fp4(key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping)
+
+
+@store_kv_fp4.register_fake
+def _(key, value, k_cache, v_cache, k_scale, v_scale, slot_mapping):
+    return None
+
+
+@custom_op(f"{_NS}::load_kv_fp4", mutates_args=())
+def load_kv_fp4(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor, v_scale: torch.Tensor,
+                slot_mapping: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    """The tokens at slot_mapping of the 4-bit cache as fp16 (k, v) [T, Hkv, 128]."""
+    return kernels.load_kv_fp4(k_cache, v_cache, k_scale, v_scale, slot_mapping)
+
+
+@load_kv_fp4.register_fake
+def _(k_cache, v_cache, k_scale, v_scale, slot_mapping):
+    shape = (slot_mapping.shape[0], k_cache.shape[1], 2 * k_cache.shape[3])
+    return (k_cache.new_empty(shape, dtype=torch.float16), k_cache.new_empty(shape, dtype=torch.float16))
+
+
+@custom_op(f"{_NS}::paged_decode_fp4", mutates_args=())
+def paged_decode_fp4(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                     v_scale: torch.Tensor, cache_seqlens: torch.Tensor, block_tables: torch.Tensor,
+                     softmax_scale: float) -> torch.Tensor:
+    """Decode attention of query [B, Hq, D] over each sequence's paged 4-bit K/V."""
+    return kernels.paged_decode_fp4(query, k_cache, v_cache, k_scale, v_scale, cache_seqlens, block_tables,
+                                    softmax_scale)
+
+
+@paged_decode_fp4.register_fake
+def _(query, k_cache, v_cache, k_scale, v_scale, cache_seqlens, block_tables, softmax_scale):
+    return query.new_empty(query.shape)
+
+
+@custom_op(f"{_NS}::paged_prefill_fp4", mutates_args=())
+def paged_prefill_fp4(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
+                      v_scale: torch.Tensor, block_tables: torch.Tensor, cu_q: torch.Tensor, kv_lens: torch.Tensor,
+                      softmax_scale: float) -> torch.Tensor:
+    """Causal attention of new tokens query [T, Hq, D] over prefix + themselves in the paged 4-bit cache."""
+    return kernels.paged_prefill_fp4(query, k_cache, v_cache, k_scale, v_scale, block_tables, cu_q, kv_lens,
+                                     softmax_scale)
+
+
+@paged_prefill_fp4.register_fake
+def _(query, k_cache, v_cache, k_scale, v_scale, block_tables, cu_q, kv_lens, softmax_scale):
+    return query.new_empty(query.shape)
+
+
+@custom_op(f"{_NS}::copy_pages", mutates_args=("cache", "scale"))
+def copy_pages(cache: torch.Tensor, scale: torch.Tensor, src: torch.Tensor, dst: torch.Tensor,
+               num_tokens: Optional[torch.Tensor] = None) -> None:
+    """Tokens [0, num_tokens[i]) of page src[i] -> page dst[i] in every plane of a paged FP8 or 4-bit cache."""
+    kernels.copy_pages(cache, scale, src, dst, num_tokens)
+
+
+@copy_pages.register_fake
+def _(cache, scale, src, dst, num_tokens=None):
+    return None
+
+
 # ------------------------------------------------------------------ sampling
 @custom_op(f"{_NS}::argmax_rows", mutates_args=())
 def argmax_rows(logits: torch.Tensor) -> torch.Tensor:
@@ -249,4 +318,5 @@ def _(logits):
 
 OPS = ("quantize_rows_fp8", "fp8_gemm", "rmsnorm", "add_rmsnorm", "rmsnorm_fp8", "add_rmsnorm_fp8", "silu_mul",
        "silu_mul_fp8", "store_kv_fp8", "qkv_post_decode", "qkv_post_prefill", "paged_decode_fp8",
-       "paged_prefill_fp8", "varlen_prefill", "argmax_rows")
+       "paged_prefill_fp8", "varlen_prefill", "argmax_rows", "store_kv_fp4", "load_kv_fp4", "paged_decode_fp4",
+       "paged_prefill_fp4", "copy_pages")

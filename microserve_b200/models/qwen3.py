@@ -7,10 +7,11 @@ reference's, so checkpoints load the same way. Two forwards exist:
 * the module path (each submodule's forward, like the reference), used when
   the linears are not FP8-quantised;
 * the fused FP8 path (Qwen3DecoderLayer.forward_fp8), used once
-  quantize_fp8_linears() ran and the KV cache is FP8. Per layer it launches:
+  quantize_fp8_linears() ran and the KV cache is FP8 or 4-bit. Per layer it launches:
     1. (residual +) RMSNorm -> FP8 rows              (input_layernorm + qkv act quant)
     2. FP8 GEMM  qkv                                  (qkv_proj)
     3. q/k RMSNorm + RoPE + FP8 KV store              (qwen3.py:49-53, attention.py:41-43)
+       (4-bit cache: the store is a kernel of its own, kernels.store_kv_fp4)
     4. attention (decode / prefill / chunk)           (attention.py:44-60)
     5. FP8 row quant of o + FP8 GEMM o_proj
     6. residual + RMSNorm -> FP8 rows                 (post_attention_layernorm + act quant)
@@ -101,12 +102,16 @@ class Qwen3Attention(nn.Module):
         ctx = get_context()
         attn = self.attn
         qkv = self.qkv_proj.forward_fp8(xq, sx)
-        want_kv = ctx.mode is AttentionMode.PREFILL
+        fp4 = attn.kv_cache_dtype == "fp4_e2m1"  # its own writer follows the prologue
+        want_kv = fp4 or ctx.mode is AttentionMode.PREFILL
         q, k, v = kernels.qkv_post(
             qkv, self.num_heads, self.num_kv_heads, self.head_dim, positions, self.rotary_emb.cos_half16,
             self.rotary_emb.sin_half16, self.q_norm.weight if self.has_qk_norm else None,
             self.k_norm.weight if self.has_qk_norm else None, self.rms_norm_eps, ctx.slot_mapping,
-            (attn.k_cache, attn.v_cache, attn.k_scale_cache, attn.v_scale_cache), want_kv=want_kv)
+            None if fp4 else (attn.k_cache, attn.v_cache, attn.k_scale_cache, attn.v_scale_cache), want_kv=want_kv)
+        if fp4:
+            kernels.store_kv_fp4(k, v, attn.k_cache, attn.v_cache, attn.k_scale_cache, attn.v_scale_cache,
+                                 ctx.slot_mapping)
         o = attn.forward_cached(q, k, v)
         oq, so = tp_quantize_rows(o.view(-1, self.q_size))
         if tpf is not None:
@@ -208,7 +213,7 @@ class Qwen3Model(nn.Module):
 
     def _fp8_ready(self) -> bool:
         a = self.layers[0].self_attn
-        return isinstance(a.qkv_proj, FP8DynamicLinear) and a.attn.kv_cache_dtype == "fp8_e4m3"
+        return isinstance(a.qkv_proj, FP8DynamicLinear) and a.attn.kv_cache_dtype in ("fp8_e4m3", "fp4_e2m1")
 
     def forward(self, input_ids: torch.Tensor, positions: torch.Tensor) -> torch.Tensor:
         hidden_states = self.embed_tokens(input_ids)
