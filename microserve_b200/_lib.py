@@ -56,7 +56,9 @@ SIGNATURES: dict[str, tuple] = {
     "ms_paged_prefill_fp8": (i32, [vp, vp, vp, vp, vp, vp, vp, vp, vp, i32, i64, i32, i32, i32, i32, i32, f32, vp]),
     "ms_store_kv_fp4": (i32, [vp, vp, i64, i64, i64, i64, i64, i32, i32, vp, vp, vp, vp, vp, i64, i32, vp]),
     "ms_load_kv_fp4": (i32, [vp, vp, vp, vp, i64, i32, i64, i32, i32, vp, vp, vp, vp]),
-    "ms_paged_decode_fp4": (i32, [vp, i64, vp, vp, vp, vp, i64, vp, vp, vp, i32, i32, i32, i32, i32, i32, f32, vp]),
+    "ms_paged_decode_fp4": (i32, [vp, i64, vp, vp, vp, vp, i64, vp, vp, vp, i32, i32, i32, i32, i32, i32, f32, vp,
+                                  sz, vp]),
+    "ms_paged_decode_fp4_workspace_size": (sz, [i32, i32, i32, i32, i32]),
     "ms_paged_prefill_fp4": (i32, [vp, i64, vp, vp, vp, vp, i64, vp, vp, vp, vp, i32, i64, i32, i32, i32, i32, i32,
                                    f32, vp]),
     "ms_copy_pages": (i32, [vp, i64, i32, vp, i64, i32, i32, i32, i32, i64, vp, vp, vp, i32, vp]),

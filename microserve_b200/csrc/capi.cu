@@ -341,10 +341,15 @@ int ms_load_kv_fp4(const void* k_cache, const void* v_cache, const void* k_scale
                     "ms_load_kv_fp4");
 }
 
+size_t ms_paged_decode_fp4_workspace_size(int B, int Hq, int Hkv, int max_blocks, int block_size) {
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || max_blocks <= 0 || block_size <= 0) return 0;
+  return ms::decode_fp4_workspace_bytes(B, Hq, Hkv, max_blocks, block_size, num_sms());
+}
+
 int ms_paged_decode_fp4(const void* q, int64_t q_token_stride, const void* k_cache, const void* v_cache,
                         const void* k_scale, const void* v_scale, int64_t num_blocks, const int32_t* seqlens,
                         const int32_t* block_tables, void* out, int B, int Hq, int Hkv, int head_dim, int block_size,
-                        int max_blocks, float softmax_scale, void* stream) {
+                        int max_blocks, float softmax_scale, void* workspace, size_t workspace_bytes, void* stream) {
   if (B < 0 || max_blocks <= 0) return fail(MS_ERR_INVALID, "ms_paged_decode_fp4: bad sizes");
   int rc = check_fp4_cache("ms_paged_decode_fp4", k_cache, v_cache, k_scale, v_scale, num_blocks, Hkv, head_dim,
                            block_size);
@@ -353,9 +358,13 @@ int ms_paged_decode_fp4(const void* q, int64_t q_token_stride, const void* k_cac
   rc = check_fp4_query("ms_paged_decode_fp4", q, q_token_stride, out, Hq, Hkv);
   if (rc != MS_OK) return rc;
   if (!seqlens || !block_tables) return fail(MS_ERR_INVALID, "ms_paged_decode_fp4: null pointer");
-  return check_cuda(ms::launch_fp4_attention(q, q_token_stride, k_cache, v_cache, k_scale, v_scale, num_blocks,
-                                             block_tables, nullptr, seqlens, out, B, B, Hq, Hkv, block_size,
-                                             max_blocks, softmax_scale, S(stream)),
+  const size_t need = ms::decode_fp4_workspace_bytes(B, Hq, Hkv, max_blocks, block_size, num_sms());
+  if (workspace_bytes < need || workspace == nullptr)
+    return fail(MS_ERR_WORKSPACE, "ms_paged_decode_fp4: workspace %zu < %zu bytes", workspace_bytes, need);
+  if (!aligned16(workspace)) return fail(MS_ERR_INVALID, "ms_paged_decode_fp4: workspace not 16-byte aligned");
+  return check_cuda(ms::launch_decode_fp4(q, q_token_stride, k_cache, v_cache, k_scale, v_scale, num_blocks, seqlens,
+                                          block_tables, out, B, Hq, Hkv, block_size, max_blocks, softmax_scale,
+                                          workspace, num_sms(), S(stream)),
                     "ms_paged_decode_fp4");
 }
 

@@ -418,10 +418,15 @@ def paged_decode_fp4(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     _int32("paged_decode_fp4", "block_tables", block_tables, B, -1)
     query, q_stride, o = _fp4_query("paged_decode_fp4", query, out)
     _on_current_device("paged_decode_fp4", query, k_cache, v_cache, k_scale, v_scale, cache_seqlens, block_tables, o)
-    check(_lib.load().ms_paged_decode_fp4(query.data_ptr(), q_stride, k_cache.data_ptr(), v_cache.data_ptr(),
-                                          k_scale.data_ptr(), v_scale.data_ptr(), NB, cache_seqlens.data_ptr(),
-                                          block_tables.data_ptr(), o.data_ptr(), B, Hq, Hkv, D, BS,
-                                          block_tables.shape[1], float(softmax_scale), stream_ptr()),
+    lib = _lib.load()
+    max_blocks = block_tables.shape[1]
+    # a workspace of its own for every call: calls on two streams, or two captured graphs, never share one
+    ws = torch.empty(lib.ms_paged_decode_fp4_workspace_size(B, Hq, Hkv, max_blocks, BS), dtype=torch.uint8,
+                     device=query.device)
+    check(lib.ms_paged_decode_fp4(query.data_ptr(), q_stride, k_cache.data_ptr(), v_cache.data_ptr(),
+                                  k_scale.data_ptr(), v_scale.data_ptr(), NB, cache_seqlens.data_ptr(),
+                                  block_tables.data_ptr(), o.data_ptr(), B, Hq, Hkv, D, BS, max_blocks,
+                                  float(softmax_scale), ws.data_ptr(), ws.numel(), stream_ptr()),
           "ms_paged_decode_fp4")
     return o
 

@@ -19,9 +19,10 @@ def _store(T=4, heads=8, dim=128, k=P, slots=P, cache=P, scale=P, blocks=4, bs=2
                                        None)
 
 
-def _decode(q=P, qs=2048, cache=P, blocks=4, lens=P, tables=P, B=2, Hq=16, Hkv=8, dim=128, bs=256, mb=4):
-    lib = _lib.load()
-    return lib.ms_paged_decode_fp4(q, qs, cache, P, P, P, blocks, lens, tables, P, B, Hq, Hkv, dim, bs, mb, 0.1, None)
+def _decode(q=P, qs=2048, cache=P, blocks=4, lens=P, tables=P, B=2, Hq=16, Hkv=8, dim=128, bs=256, mb=4,
+            ws=P, wb=1 << 30):
+    return _lib.load().ms_paged_decode_fp4(q, qs, cache, P, P, P, blocks, lens, tables, P, B, Hq, Hkv, dim, bs, mb,
+                                           0.1, ws, wb, None)
 
 
 def _prefill(q=P, qs=2048, cache=P, blocks=4, tables=P, cu=P, n=2, T=9, Hq=16, Hkv=8, dim=128, bs=256, mb=4):
@@ -47,6 +48,8 @@ INVALID, UNSUPPORTED = _lib.MS_ERR_INVALID, _lib.MS_ERR_UNSUPPORTED
     (_decode, dict(Hq=72), UNSUPPORTED), (_decode, dict(dim=96), UNSUPPORTED), (_decode, dict(bs=32), UNSUPPORTED),
     (_decode, dict(q=P + 2), INVALID), (_decode, dict(qs=2000), INVALID), (_decode, dict(qs=1024), INVALID),
     (_decode, dict(lens=None), INVALID), (_decode, dict(tables=None), INVALID), (_decode, dict(mb=0), INVALID),
+    (_decode, dict(ws=None), _lib.MS_ERR_WORKSPACE), (_decode, dict(wb=100), _lib.MS_ERR_WORKSPACE),
+    (_decode, dict(ws=P + 4), INVALID),
     (_prefill, dict(n=0), 0), (_prefill, dict(T=0), 0), (_prefill, dict(T=1 << 31), INVALID),
     (_prefill, dict(Hq=9), UNSUPPORTED), (_prefill, dict(cu=None), INVALID), (_prefill, dict(q=None), INVALID),
     (_prefill, dict(bs=100), UNSUPPORTED), (_prefill, dict(Hkv=0), INVALID),
