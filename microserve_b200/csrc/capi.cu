@@ -382,9 +382,9 @@ int ms_paged_prefill_fp4(const void* q, int64_t q_token_stride, const void* k_ca
   rc = check_fp4_query("ms_paged_prefill_fp4", q, q_token_stride, out, Hq, Hkv);
   if (rc != MS_OK) return rc;
   if (!block_tables || !cu_q || !kv_lens) return fail(MS_ERR_INVALID, "ms_paged_prefill_fp4: null pointer");
-  return check_cuda(ms::launch_fp4_attention(q, q_token_stride, k_cache, v_cache, k_scale, v_scale, num_blocks,
-                                             block_tables, cu_q, kv_lens, out, num_seqs, (int)total_q, Hq, Hkv,
-                                             block_size, max_blocks, softmax_scale, S(stream)),
+  return check_cuda(ms::launch_prefill_fp4(q, q_token_stride, k_cache, v_cache, k_scale, v_scale, num_blocks,
+                                           block_tables, cu_q, kv_lens, out, num_seqs, (int)total_q, Hq, Hkv,
+                                           block_size, max_blocks, softmax_scale, S(stream)),
                     "ms_paged_prefill_fp4");
 }
 
