@@ -67,7 +67,10 @@ int check_fp4_cache(const char* what, const void* k_cache, const void* v_cache, 
 }
 
 // Query / output layout of the attentions over the 4-bit cache.
-int check_fp4_query(const char* what, const void* q, int64_t q_stride, const void* out, int Hq, int Hkv) {
+int check_fp4_query(const char* what, const void* q, int64_t q_stride, const void* out, int Hq, int Hkv,
+                    float softmax_scale) {
+  if (!(softmax_scale > 0.f) || softmax_scale > 3e38f)
+    return fail(MS_ERR_INVALID, "%s: softmax_scale must be a positive finite number", what);
   if (Hq <= 0 || Hq % Hkv != 0 || Hq / Hkv > 8)
     return fail(MS_ERR_UNSUPPORTED, "%s: Hq=%d Hkv=%d unsupported (Hq a multiple of Hkv, at most 8 per kv head)", what,
                 Hq, Hkv);
@@ -99,8 +102,10 @@ int ms_get_device_status(int* status, void* stream) {
                                             S(stream));
   if (e == cudaSuccess)
     e = cudaMemcpyToSymbolAsync(ms::g_device_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, S(stream));
+  int own = 0;
+  if (e == cudaSuccess) e = ms::prefill_fp4_take_status(&own, S(stream));
   if (e == cudaSuccess) e = cudaStreamSynchronize(S(stream));
-  *status = host;
+  *status = host != 0 ? host : own;
   return check_cuda(e, "ms_get_device_status");
 }
 
@@ -355,7 +360,7 @@ int ms_paged_decode_fp4(const void* q, int64_t q_token_stride, const void* k_cac
                            block_size);
   if (rc != MS_OK) return rc;
   if (B == 0) return MS_OK;
-  rc = check_fp4_query("ms_paged_decode_fp4", q, q_token_stride, out, Hq, Hkv);
+  rc = check_fp4_query("ms_paged_decode_fp4", q, q_token_stride, out, Hq, Hkv, softmax_scale);
   if (rc != MS_OK) return rc;
   if (!seqlens || !block_tables) return fail(MS_ERR_INVALID, "ms_paged_decode_fp4: null pointer");
   const size_t need = ms::decode_fp4_workspace_bytes(B, Hq, Hkv, max_blocks, block_size, num_sms());
@@ -379,7 +384,7 @@ int ms_paged_prefill_fp4(const void* q, int64_t q_token_stride, const void* k_ca
                            block_size);
   if (rc != MS_OK) return rc;
   if (num_seqs == 0 || total_q == 0) return MS_OK;
-  rc = check_fp4_query("ms_paged_prefill_fp4", q, q_token_stride, out, Hq, Hkv);
+  rc = check_fp4_query("ms_paged_prefill_fp4", q, q_token_stride, out, Hq, Hkv, softmax_scale);
   if (rc != MS_OK) return rc;
   if (!block_tables || !cu_q || !kv_lens) return fail(MS_ERR_INVALID, "ms_paged_prefill_fp4: null pointer");
   return check_cuda(ms::launch_prefill_fp4(q, q_token_stride, k_cache, v_cache, k_scale, v_scale, num_blocks,
@@ -577,7 +582,9 @@ int ms_fp8_gemm_rowpar_ar_rmsnorm(const void* xq, const float* sx, const void* w
 int ms_set_wait_limit(uint64_t ns) {
   if (ns == 0) return fail(MS_ERR_INVALID, "ms_set_wait_limit: limit must be > 0");
   const unsigned long long v = ns;
-  return check_cuda(cudaMemcpyToSymbol(ms::g_wait_limit_ns, &v, sizeof(v)), "ms_set_wait_limit");
+  cudaError_t e = cudaMemcpyToSymbol(ms::g_wait_limit_ns, &v, sizeof(v));
+  if (e == cudaSuccess) e = ms::prefill_fp4_set_wait_limit(v);
+  return check_cuda(e, "ms_set_wait_limit");
 }
 
 int ms_row_amax(const void* x, int64_t ldx, int64_t M, int64_t K, float* amax, void* stream) {

@@ -7,13 +7,15 @@
 // a (token, query head) pair of the G = Hq / Hkv heads that share a kv head, over tiles of
 // 128 keys that both read:
 //   warps 0-3, 4-7   softmax of tile 0 / 1: a thread owns a row. It reads its 128 scores from
-//                    TMEM, writes the weights back over them as f16, and keeps the
+//                    TMEM, writes the weights over them as f16, and keeps the
 //                    row's maximum and sum (fp32). While one tile's softmax runs, the
 //                    tensor core works for the other.
-//   warps 8-10       decode K and V codes to f16 in shared memory (128-byte swizzle), a
+//   warps 8-14       decode K and V codes to f16 in shared memory (128-byte swizzle), a
 //                    ring of kSlots 32 KB slots in the order K0 V0 K1 V1 ..., 32 keys a
-//                    warp at a time; the next codes are fetched into registers meanwhile.
-//   warp 11          allocates TMEM; one thread issues S = Q K^T (both operands K-major in
+//                    warp at a time (three warps, with the next codes prefetched, could not
+//                    keep up: 1.76 ms against 1.01 ms without decoding, 2048 queries on
+//                    30720 tokens).
+//   warp 15          allocates TMEM; one thread issues S = Q K^T (both operands K-major in
 //                    shared memory) and O += P V (P from TMEM, V as it lies in the cache:
 //                    MN-major).
 // Softmax in the exp2 domain against a lazy reference: weights are 2^(s - m) for a reference
@@ -24,6 +26,7 @@
 // V rows behind the sequence's end and rows of bad pages are written as zeros, and a NaN group
 // of V as zeros too, because a zero weight does not hide a NaN from the product: the first
 // key with a NaN is kept per 16 elements, and the rows that see it get NaN at the end.
+#define MS_WHOLE_PROGRAM  // setmaxnreg below
 #include <mutex>
 
 #include "fp4_kv.cuh"
@@ -39,9 +42,12 @@ constexpr int kHalf = 128 * 128;              // 128 rows x 64 elements of f16, 
 constexpr int kSlotBytes = 2 * kHalf;         // a K or V tile
 constexpr int kSlots = 5;
 constexpr int kQBytes = 2 * 2 * kHalf;        // two tiles
-constexpr int kDecodeWarps = 3;
+constexpr int kDecodeWarps = 7;
 constexpr int kThreads = (8 + kDecodeWarps + 1) * 32;
 constexpr int kMmaWarp = 8 + kDecodeWarps;
+// Registers: 512 threads start with 128 each; the decode and MMA warps hand some to softmax.
+constexpr int kSoftmaxRegs = 184, kDecodeRegs = 72;
+static_assert(256 * (kSoftmaxRegs + kDecodeRegs) <= 65536, "register shares");
 constexpr int kSmemBytes = kQBytes + kSlots * kSlotBytes + 1024 /* alignment */;
 constexpr int kTmemCols = 512;                // S0 S1 O0 O1, 128 columns each
 constexpr float kLog2e = 1.4426950408889634f;
@@ -112,20 +118,52 @@ __device__ __forceinline__ void tmem_st16(uint32_t addr, const uint32_t (&r)[16]
       "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
       : "memory");
 }
-__device__ __forceinline__ void tmem_st32(uint32_t addr, const float (&v)[32]) {
-  const uint32_t* r = reinterpret_cast<const uint32_t*>(v);
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,"
-      "%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(addr),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-      "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
-      "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
-      "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-      : "memory");
+// Scores of keys that the row does not see (bits of `seen` not set).
+__device__ __forceinline__ void hide(float (&x)[32], uint32_t seen) {
+#pragma unroll
+  for (int i = 0; i < 32; ++i)
+    if (!((seen >> i) & 1u)) x[i] = -INFINITY;
+}
+__device__ __forceinline__ float max32(const float (&x)[32], float m) {
+  float t[4] = {m, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+  for (int i = 0; i < 32; i += 8)
+#pragma unroll
+    for (int u = 0; u < 4; ++u) t[u] = fmaxf(fmaxf(t[u], x[i + 2 * u]), x[i + 2 * u + 1]);
+  return fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
 }
 
 // Every thread of the CTA, from the ends of the roles.
 __device__ __forceinline__ void role_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); }
+
+__device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&v)[16]) {
+  uint32_t* r = reinterpret_cast<uint32_t*>(v);
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
+        "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+      : "r"(addr));
+}
+
+// Pairs of floats in one 64-bit register: one instruction for two.
+__device__ __forceinline__ uint64_t f32x2(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
 
 struct PrefillArgs {
   const __half* q;  // [T, Hq, D], token stride q_ts elements
@@ -234,6 +272,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_fp4_kernel(const __grid_c
 
   if (item.seq >= 0 && warp < 8) {
     // ------------------------------------------------------------------ softmax
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     const int t = warp >> 2;                                  // tile
     const int row = (warp & 3) * 32 + lane;                   // TMEM lane
     const int tt = t * tpt + row / G, h = row % G;            // token of the CTA, head of the group
@@ -284,32 +323,16 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_fp4_kernel(const __grid_c
           }
           masked = true;
         }
-        // ---- maximum -------------------------------------------------------------------
-        float mx = -INFINITY;
+        // ---- the row's 128 scores, and their maximum --------------------------------------------
+        float v[4][32];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          float v[32];
-          tmem_ld32(s_addr + 32 * c, v);
-          tmem_ld_wait();
-          if (masked) {
+        for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + 32 * c, v[c]);
+        tmem_ld_wait();
+        if (masked) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (!((seen[c] >> i) & 1u)) v[i] = a.scale_log2 < 0.f ? INFINITY : -INFINITY;
-          }
-          if (a.scale_log2 < 0.f) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i) mx = fmaxf(mx, v[i] * a.scale_log2);
-          } else {
-            float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-            for (int i = 0; i < 32; i += 4) {
-#pragma unroll
-              for (int u = 0; u < 4; ++u) m4[u] = fmaxf(m4[u], v[i + u]);
-            }
-            const float top = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-            mx = fmaxf(mx, top == -INFINITY ? top : top * a.scale_log2);
-          }
+          for (int c = 0; c < 4; ++c) hide(v[c], seen[c]);
         }
+        const float mx = max32(v[3], max32(v[2], max32(v[1], max32(v[0], -INFINITY)))) * a.scale_log2;
         // ---- the reference moves when some row's maximum is far above it ---------------------
         const bool far = mx - kPScaleLog2 > m + kMove || (m == -INFINITY && mx > -INFINITY);
         if (__any_sync(0xffffffffu, far)) {
@@ -324,41 +347,39 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_fp4_kernel(const __grid_c
             }
             tc_fence_after();
 #pragma unroll
-            for (int c = 0; c < 4; ++c) {
-              float v[32];
-              tmem_ld32(o_addr + 32 * c, v);
+            for (int c = 0; c < 8; ++c) {
+              float o[16];
+              tmem_ld16(o_addr + 16 * c, o);
               tmem_ld_wait();
 #pragma unroll
-              for (int i = 0; i < 32; ++i) v[i] *= al;
-              tmem_st32(o_addr + 32 * c, v);
+              for (int i = 0; i < 16; ++i) o[i] *= al;
+              tmem_st16(o_addr + 16 * c, *reinterpret_cast<uint32_t(*)[16]>(o));
             }
             tmem_st_wait();
           }
         }
         // ---- weights, f16, over the scores ----------------------------------------------------
-        const float mu = m == -INFINITY ? 0.f : m;
+        const float neg = m == -INFINITY ? 0.f : -m;
+        const uint64_t sc2 = f32x2(a.scale_log2, a.scale_log2), neg2 = f32x2(neg, neg);
+        uint64_t sum[2] = {0, 0};
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
-          float v[32];
-          tmem_ld32(s_addr + 32 * c, v);
-          tmem_ld_wait();
-#pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = ex2(fmaf(v[i], a.scale_log2, -mu));
-          if (masked) {
-#pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (!((seen[c] >> i) & 1u)) v[i] = 0.f;
-          }
-          float l4[4] = {0.f, 0.f, 0.f, 0.f};
           uint32_t p[16];
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
-            l4[i & 2] += v[i];
-            l4[(i & 2) + 1] += v[i + 1];
-            p[i >> 1] = pack_h2(v[i], v[i + 1]);
+            float x0, x1;
+            unpack2(fma2(f32x2(v[c][i], v[c][i + 1]), sc2, neg2), x0, x1);
+            x0 = ex2(x0);
+            x1 = ex2(x1);
+            sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], f32x2(x0, x1));
+            p[i >> 1] = pack_h2(x0, x1);
           }
-          l += (l4[0] + l4[1]) + (l4[2] + l4[3]);
           tmem_st16(s_addr + 16 * c, p);
+        }
+        {
+          float x0, x1;
+          unpack2(add2(sum[0], sum[1]), x0, x1);
+          l += x0 + x1;
         }
         tmem_st_wait();
         tc_fence_before();
@@ -399,7 +420,9 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_fp4_kernel(const __grid_c
     } else {
       role_sync();
     }
-  } else if (item.seq >= 0 && warp < kMmaWarp) {
+  } else if (item.seq >= 0) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kDecodeRegs));
+    if (warp < kMmaWarp) {
     // ------------------------------------------------------------------ decode of K and V
     const int lr = lane >> 2, lc = lane & 3;
     // unit u: 32 keys (u % 4) of slot number n = u / 4, which is K (n even) or V (odd) of tile n / 2
@@ -424,14 +447,15 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_fp4_kernel(const __grid_c
         x.s[i] = __ldg(reinterpret_cast<const uint16_t*>(scales + i * 8 * kFp4ScaleBytes));
       }
     };
-    Codes cur, nxt;
-    bool cur_live = false, nxt_live = false;
+    Codes cur;
+    bool cur_live = false;
     const int total = 8 * n_kv;
-    if (warp - 8 < total) fetch(warp - 8, nxt, nxt_live);
+    // A warp does not write every slot, so it may skip a use of one: it waits by parity all the
+    // same, because its previous unit lay at most two slots back and waited for a release that
+    // comes after the one before last of this slot.
+    static_assert(kDecodeWarps <= 8 && kSlots > 2, "a warp's units are at most two slots apart");
     for (int u = warp - 8; u < total; u += kDecodeWarps) {
-      cur = nxt;
-      cur_live = nxt_live;
-      if (u + kDecodeWarps < total) fetch(u + kDecodeWarps, nxt, nxt_live);
+      fetch(u, cur, cur_live);
       const int n = u >> 2, slot = n % kSlots;
       if (!mbar_wait(&empty[slot], ((n / kSlots) & 1) ^ 1)) break;
       unsigned char* dst = s_kv + slot * kSlotBytes + (lc >> 1) * kHalf;
@@ -478,7 +502,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_fp4_kernel(const __grid_c
     }
     __syncwarp();
     role_sync();
-  } else if (item.seq >= 0) {
+    } else {
     // ------------------------------------------------------------------ MMA issue
     if (lane == 0 && n_kv > 0) {
       const uint32_t kv0 = smem_u32(s_kv), q0 = smem_u32(s_q);
@@ -527,6 +551,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_fp4_kernel(const __grid_c
     }
     __syncwarp();
     role_sync();
+    }
   }
   tc_fence_before();
   __syncthreads();
@@ -537,6 +562,18 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_fp4_kernel(const __grid_c
 }
 
 }  // namespace
+
+cudaError_t prefill_fp4_take_status(int* host, cudaStream_t stream) {
+  static const int zero = 0;
+  cudaError_t e = cudaMemcpyFromSymbolAsync(host, g_device_status, sizeof(int), 0, cudaMemcpyDeviceToHost, stream);
+  if (e == cudaSuccess)
+    e = cudaMemcpyToSymbolAsync(g_device_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, stream);
+  return e;
+}
+
+cudaError_t prefill_fp4_set_wait_limit(unsigned long long ns) {
+  return cudaMemcpyToSymbol(g_wait_limit_ns, &ns, sizeof(ns));
+}
 
 cudaError_t launch_prefill_fp4(const void* q, int64_t q_ts, const void* k_cache, const void* v_cache,
                                const void* k_scale, const void* v_scale, int64_t num_blocks,

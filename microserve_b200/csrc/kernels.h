@@ -54,6 +54,9 @@ cudaError_t launch_decode_fp4(const void* q, int64_t q_ts, const void* k_cache, 
                               const void* k_scale, const void* v_scale, int64_t num_blocks, const int32_t* seqlens,
                               const int32_t* block_tables, void* out, int B, int Hq, int Hkv, int block_size,
                               int max_blocks, float softmax_scale, void* workspace, int num_sms, cudaStream_t stream);
+// The status word and wait limit of fp4_prefill_attn.cu (common.cuh: MS_WHOLE_PROGRAM).
+cudaError_t prefill_fp4_take_status(int* host, cudaStream_t stream);
+cudaError_t prefill_fp4_set_wait_limit(unsigned long long ns);
 cudaError_t launch_prefill_fp4(const void* q, int64_t q_ts, const void* k_cache, const void* v_cache,
                                const void* k_scale, const void* v_scale, int64_t num_blocks,
                                const int32_t* block_tables, const int32_t* cu_q, const int32_t* kv_lens, void* out,

@@ -20,14 +20,15 @@ def _store(T=4, heads=8, dim=128, k=P, slots=P, cache=P, scale=P, blocks=4, bs=2
 
 
 def _decode(q=P, qs=2048, cache=P, blocks=4, lens=P, tables=P, B=2, Hq=16, Hkv=8, dim=128, bs=256, mb=4,
-            ws=P, wb=1 << 30):
+            ws=P, wb=1 << 30, scale=0.1):
     return _lib.load().ms_paged_decode_fp4(q, qs, cache, P, P, P, blocks, lens, tables, P, B, Hq, Hkv, dim, bs, mb,
-                                           0.1, ws, wb, None)
+                                           scale, ws, wb, None)
 
 
-def _prefill(q=P, qs=2048, cache=P, blocks=4, tables=P, cu=P, n=2, T=9, Hq=16, Hkv=8, dim=128, bs=256, mb=4):
+def _prefill(q=P, qs=2048, cache=P, blocks=4, tables=P, cu=P, n=2, T=9, Hq=16, Hkv=8, dim=128, bs=256, mb=4,
+             scale=0.1):
     return _lib.load().ms_paged_prefill_fp4(q, qs, cache, P, P, P, blocks, tables, cu, P, P, n, T, Hq, Hkv, dim, bs,
-                                            mb, 0.1, None)
+                                            mb, scale, None)
 
 
 def _copy(cache=P, cs=1 << 30, row=1024, scale=P, ss=1 << 30, srow=32, planes=2, outer=1, bs=256, pages=8, src=P,
@@ -49,7 +50,8 @@ INVALID, UNSUPPORTED = _lib.MS_ERR_INVALID, _lib.MS_ERR_UNSUPPORTED
     (_decode, dict(q=P + 2), INVALID), (_decode, dict(qs=2000), INVALID), (_decode, dict(qs=1024), INVALID),
     (_decode, dict(lens=None), INVALID), (_decode, dict(tables=None), INVALID), (_decode, dict(mb=0), INVALID),
     (_decode, dict(ws=None), _lib.MS_ERR_WORKSPACE), (_decode, dict(wb=100), _lib.MS_ERR_WORKSPACE),
-    (_decode, dict(ws=P + 4), INVALID),
+    (_decode, dict(ws=P + 8), INVALID), (_decode, dict(scale=0.0), INVALID), (_decode, dict(scale=-1.0), INVALID),
+    (_decode, dict(scale=float("nan")), INVALID), (_prefill, dict(scale=float("inf")), INVALID),
     (_prefill, dict(n=0), 0), (_prefill, dict(T=0), 0), (_prefill, dict(T=1 << 31), INVALID),
     (_prefill, dict(Hq=9), UNSUPPORTED), (_prefill, dict(cu=None), INVALID), (_prefill, dict(q=None), INVALID),
     (_prefill, dict(bs=100), UNSUPPORTED), (_prefill, dict(Hkv=0), INVALID),
