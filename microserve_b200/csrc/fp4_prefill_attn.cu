@@ -4,20 +4,23 @@
 //
 // Tensor bound (4 * 128 * Hq operations per visible pair), so both products run on tcgen05
 // with fp32 accumulators in TMEM. One CTA handles two tiles of 128 query rows, a row being
-// a (token, query head) pair of the G = Hq / Hkv heads that share a kv head, over tiles of
-// 128 keys that both read:
-//   warps 0-3, 4-7   softmax of tile 0 / 1: a thread owns a row. It reads its 128 scores from
-//                    TMEM, writes the weights over them as f16, and keeps the
-//                    row's maximum and sum (fp32). While one tile's softmax runs, the
-//                    tensor core works for the other.
-//   warps 8-14       decode K and V codes to f16 in shared memory (128-byte swizzle), a
-//                    ring of kSlots 32 KB slots in the order K0 V0 K1 V1 ..., 32 keys a
-//                    warp at a time (three warps, with the next codes prefetched, could not
-//                    keep up: 1.76 ms against 1.01 ms without decoding, 2048 queries on
-//                    30720 tokens).
-//   warp 15          allocates TMEM; one thread issues S = Q K^T (both operands K-major in
-//                    shared memory) and O += P V (P from TMEM, V as it lies in the cache:
-//                    MN-major).
+// a (token, query head) pair of the G = Hq / Hkv heads that share a kv head, over steps of
+// 64 keys that both read:
+//   warps 0-3, 4-7   softmax of tile 0 / 1: a thread owns a row. It reads its 64 scores of a
+//                    step from TMEM, writes the weights over them as f16, and keeps the row's
+//                    maximum and sum (fp32).
+//   warps 8-13       decode K and V codes to f16 in shared memory (128-byte swizzle), a
+//                    ring of kSlots 16 KB slots in the order K0 V0 K1 V1 ..., a warp a slot:
+//                    the fence between its stores and the tensor core's reads and the
+//                    barriers cost as much as 16 keys' work (16 keys a turn: 1.34 ms).
+//   warps 14, 15     each issues one tile's S = Q K^T (both in shared memory, K-major) and
+//                    O += P V (P from TMEM, V as it lies in the cache: MN-major). One warp for
+//                    both tiles spends 1.6 thousand cycles a step on waits and issue, the
+//                    tensor core needs 1.24. Warp 15 allocates TMEM.
+// The scores are double-buffered (TMEM: two tiles x two S of 64 columns, two O of 128), so S of
+// the next step is there when a softmax ends and the chain S -> softmax -> P V of a tile never
+// stalls its softmax warps: with one S a tile (128 keys a step, or 64 and Q in TMEM) the
+// chain's latencies showed, 1.11 and 1.25 ms for 2048 queries on 30720 tokens.
 // Softmax in the exp2 domain against a lazy reference: weights are 2^(s - m) for a reference
 // m that moves, with a rescale of O in TMEM, only when a row's maximum exceeds it by 8 or
 // more. Weights are rounded to f16 for the second product (2^-11 relative; the first
@@ -37,26 +40,28 @@ namespace {
 
 constexpr int kD = kFp4Dim;
 constexpr int kRows = 128;                    // query rows of a tile (MMA M)
-constexpr int kKeys = 128;                    // keys of a tile
-constexpr int kHalf = 128 * 128;              // 128 rows x 64 elements of f16, 128-byte swizzled
-constexpr int kSlotBytes = 2 * kHalf;         // a K or V tile
-constexpr int kSlots = 5;
-constexpr int kQBytes = 2 * 2 * kHalf;        // two tiles
-constexpr int kDecodeWarps = 7;
-constexpr int kThreads = (8 + kDecodeWarps + 1) * 32;
-constexpr int kMmaWarp = 8 + kDecodeWarps;
-// Registers: 512 threads start with 128 each; the decode and MMA warps hand some to softmax.
-constexpr int kSoftmaxRegs = 184, kDecodeRegs = 72;
-static_assert(256 * (kSoftmaxRegs + kDecodeRegs) <= 65536, "register shares");
+constexpr int kKeys = 64;                     // keys of a step
+constexpr int kHalf = kKeys * 128;            // 64 keys x 64 elements of f16, 128-byte swizzled
+constexpr int kSlotBytes = 2 * kHalf;         // K or V of a step
+constexpr int kSlots = 10;
+constexpr int kDecodeWarps = 6;
+constexpr int kThreads = (8 + kDecodeWarps + 2) * 32;
+constexpr int kMmaWarp = 8 + kDecodeWarps;     // of tile 0; the next one is tile 1's
+
+constexpr int kQHalf = kRows * 128;             // 128 rows x 64 elements of Q, 128-byte swizzled
+constexpr int kQBytes = 2 * 2 * kQHalf;        // two tiles
 constexpr int kSmemBytes = kQBytes + kSlots * kSlotBytes + 1024 /* alignment */;
-constexpr int kTmemCols = 512;                // S0 S1 O0 O1, 128 columns each
+constexpr int kTmemCols = 512;
+constexpr int kColO = 256;                    // first column of O0; S of tile t, step j: t * 128 + (j & 1) * 64
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kPScaleLog2 = 6.f;            // weights up to 2^(6 + 8)
 constexpr float kMove = 8.f;                  // the reference moves when a maximum exceeds it by this
 
-// tcgen05 instruction descriptor: D f32, A and B f16, M = N = 128; V is MN-major (bit 16)
+// tcgen05 instruction descriptors: D f32, A and B f16, M = 128, N = 64 keys / 128 elements; V is
+// MN-major (bit 16)
 constexpr uint32_t kIdescQK = (1u << 4) | ((uint32_t)(kKeys >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
-constexpr uint32_t kIdescPV = kIdescQK | (1u << 16);
+constexpr uint32_t kIdescPV =
+    (1u << 4) | (1u << 16) | ((uint32_t)(kD >> 3) << 17) | ((uint32_t)(kRows >> 4) << 24);
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -77,21 +82,33 @@ __device__ __forceinline__ uint64_t desc_base(uint32_t addr, uint32_t lbo) {
          ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
 }
 
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accum) {
+__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t da, uint64_t db, uint32_t idesc, uint32_t accum,
+                                       uint32_t lead) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(da), "l"(db), "r"(idesc), "r"(accum));
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+      "l"(da), "l"(db), "r"(idesc), "r"(accum), "r"(lead));
 }
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t db, uint32_t idesc, uint32_t accum) {
+__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t db, uint32_t idesc, uint32_t accum, uint32_t lead) {
   asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(db), "r"(idesc), "r"(accum));
+      "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+      "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+      "r"(a), "l"(db), "r"(idesc), "r"(accum), "r"(lead));
 }
-__device__ __forceinline__ void mma_commit(uint64_t* bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
-               : "memory");
+__device__ __forceinline__ void mma_commit(uint64_t* bar, uint32_t lead) {
+  asm volatile(
+      "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+      "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+      "r"(lead)
+      : "memory");
+}
+// One lane of the (converged) warp.
+__device__ __forceinline__ uint32_t elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r;
 }
 __device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
@@ -183,16 +200,9 @@ struct Item {
   int seq, tok0;  // first query token of the CTA within its sequence
 };
 
-// The codes of one thread's part of a K or V tile: rows lane / 4 + 8 i of its warp's 32 keys,
-// elements 32 (lane % 4) .. + 32 of each.
-struct Codes {
-  uint4 c[4];
-  uint32_t s[4];  // two scale bytes
-};
-
 __global__ void __launch_bounds__(kThreads, 1) prefill_fp4_kernel(const __grid_constant__ PrefillArgs a) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
-  __shared__ uint64_t q_full[2], full[kSlots], empty[kSlots], s_full[2], p_ready[2], pv_done[2];
+  __shared__ uint64_t q_full[2], full[kSlots], empty[kSlots], s_full[2][2], p_ready[2][2], pv_done[2];
   __shared__ uint32_t s_tmem;
   __shared__ Item s_item;
   __shared__ int s_nan[8];  // first key whose V group is NaN, per 16 elements
@@ -206,7 +216,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_fp4_kernel(const __grid_c
   const int G = a.G, tpt = kRows / G;  // tokens per tile
   const int kvh = blockIdx.y;
 
-  if (warp == kMmaWarp) {
+  if (warp == kMmaWarp + 1) {
     // this CTA's sequence and first token: a scan of the sequences' numbers of CTAs
     int left = blockIdx.x, found = -1, tok0 = 0;
     for (int s0 = 0; s0 < a.num_seqs && found < 0; s0 += 32) {
@@ -232,14 +242,17 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_fp4_kernel(const __grid_c
     if (lane == 0) {
       s_item = Item{found, tok0};
       s_bad = 0;
+      const int ql = found < 0 ? 0 : a.cu_q[found + 1] - a.cu_q[found];
       for (int i = 0; i < kSlots; ++i) {
-        mbar_init(&full[i], 4);
-        mbar_init(&empty[i], 1);
+        mbar_init(&full[i], 1);
+        mbar_init(&empty[i], ql - tok0 > tpt ? 2 : 1);  // the products of every tile have read the slot
       }
       for (int i = 0; i < 2; ++i) {
         mbar_init(&q_full[i], 128);
-        mbar_init(&s_full[i], 1);
-        mbar_init(&p_ready[i], 128);
+        for (int h = 0; h < 2; ++h) {  // the steps' parities
+          mbar_init(&s_full[i][h], 1);
+          mbar_init(&p_ready[i][h], 128);
+        }
         mbar_init(&pv_done[i], 1);
       }
       fence_barrier_init();
@@ -272,67 +285,62 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_fp4_kernel(const __grid_c
 
   if (item.seq >= 0 && warp < 8) {
     // ------------------------------------------------------------------ softmax
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     const int t = warp >> 2;                                  // tile
     const int row = (warp & 3) * 32 + lane;                   // TMEM lane
     const int tt = t * tpt + row / G, h = row % G;            // token of the CTA, head of the group
     const bool valid = row < tpt * G && tt < n_tok;
     const int lim = valid ? min(prefix + item.tok0 + tt, kv_len - 1) : -1;  // last visible key
     if (t < tiles) {
+      const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+      const uint32_t o_addr = lane_base + kColO + t * kD;
       // Q: 16 lanes a row
       const int tw = threadIdx.x & 127;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
         const int r = (tw >> 4) + 8 * i, ch = tw & 15;
         const int rt = t * tpt + r / G;
-        uint4 v = make_uint4(0, 0, 0, 0);
+        uint4 x = make_uint4(0, 0, 0, 0);
         if (r < tpt * G && rt < n_tok)
-          v = *reinterpret_cast<const uint4*>(a.q + (int64_t)(q_start + item.tok0 + rt) * a.q_ts +
+          x = *reinterpret_cast<const uint4*>(a.q + (int64_t)(q_start + item.tok0 + rt) * a.q_ts +
                                               (kvh * G + r % G) * kD + ch * 8);
-        *reinterpret_cast<uint4*>(s_q + (t * 2 + (ch >> 3)) * kHalf + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = v;
+        *reinterpret_cast<uint4*>(s_q + (t * 2 + (ch >> 3)) * kQHalf + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = x;
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(&q_full[t]);
-
-      const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-      const uint32_t s_addr = lane_base + t * 128, o_addr = lane_base + 256 + t * 128;
       int low = lim;  // smallest limit of the warp: tiles below it need no mask
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) low = min(low, __shfl_xor_sync(0xffffffffu, low, o));
       float m = -INFINITY, l = 0.f;  // reference (log2 units, less kPScaleLog2) and sum
       bool ok = true;
       for (int j = 0; j < n_kv; ++j) {
-        if (!mbar_wait(&s_full[t], j & 1)) {
+        if (!mbar_wait(&s_full[t][j & 1], (j >> 1) & 1)) {
           ok = false;
           break;
         }
         tc_fence_after();
         const int kbase = j * kKeys;
-        uint32_t seen[4];  // visible keys of the tile, a bit each
+        const uint32_t s_addr = lane_base + t * 128 + (j & 1) * kKeys;
+        const bool masked = kbase + kKeys - 1 > low || *reinterpret_cast<volatile int*>(&s_bad) != 0;
+        // ---- the row's 64 scores, and their maximum ---------------------------------------------
+        float v[2][32];
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          const int k0 = kbase + 32 * c, n = lim - k0 + 1;
-          seen[c] = n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u);
-        }
-        bool masked = kbase + kKeys - 1 > low;
-        if (*reinterpret_cast<volatile int*>(&s_bad) != 0) {  // rare: leave out the keys of bad pages
-          for (int c = 0; c < 4; ++c) {
-            const int pg = (kbase + 32 * c) / a.block_size;
-            const int64_t blk = pg < a.max_blocks ? table[pg] : -1;
-            if (blk < 0 || blk >= a.num_blocks) seen[c] = 0;
-          }
-          masked = true;
-        }
-        // ---- the row's 128 scores, and their maximum --------------------------------------------
-        float v[4][32];
-#pragma unroll
-        for (int c = 0; c < 4; ++c) tmem_ld32(s_addr + 32 * c, v[c]);
+        for (int c = 0; c < 2; ++c) tmem_ld32(s_addr + 32 * c, v[c]);
         tmem_ld_wait();
         if (masked) {
+          const bool bad = *reinterpret_cast<volatile int*>(&s_bad) != 0;
 #pragma unroll
-          for (int c = 0; c < 4; ++c) hide(v[c], seen[c]);
+          for (int c = 0; c < 2; ++c) {
+            const int k0 = kbase + 32 * c, n = lim - k0 + 1;  // keys of these 32 that the row sees
+            uint32_t seen = n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u);
+            if (bad) {  // rare: leave out the keys of bad pages
+              const int pg = k0 / a.block_size;
+              const int64_t blk = pg < a.max_blocks ? table[pg] : -1;
+              if (blk < 0 || blk >= a.num_blocks) seen = 0;
+            }
+            hide(v[c], seen);
+          }
         }
-        const float mx = max32(v[3], max32(v[2], max32(v[1], max32(v[0], -INFINITY)))) * a.scale_log2;
+        const float mx = max32(v[1], max32(v[0], -INFINITY)) * a.scale_log2;
         // ---- the reference moves when some row's maximum is far above it ---------------------
         const bool far = mx - kPScaleLog2 > m + kMove || (m == -INFINITY && mx > -INFINITY);
         if (__any_sync(0xffffffffu, far)) {
@@ -363,7 +371,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_fp4_kernel(const __grid_c
         const uint64_t sc2 = f32x2(a.scale_log2, a.scale_log2), neg2 = f32x2(neg, neg);
         uint64_t sum[2] = {0, 0};
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {
+        for (int c = 0; c < 2; ++c) {
           uint32_t p[16];
 #pragma unroll
           for (int i = 0; i < 32; i += 2) {
@@ -376,14 +384,14 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_fp4_kernel(const __grid_c
           }
           tmem_st16(s_addr + 16 * c, p);
         }
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&p_ready[t][j & 1]);
         {
           float x0, x1;
           unpack2(add2(sum[0], sum[1]), x0, x1);
           l += x0 + x1;
         }
-        tmem_st_wait();
-        tc_fence_before();
-        mbar_arrive(&p_ready[t]);
       }
       // ---- O / l ----------------------------------------------------------------------------------
       if (ok && n_kv > 0) {
@@ -421,79 +429,75 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_fp4_kernel(const __grid_c
       role_sync();
     }
   } else if (item.seq >= 0) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kDecodeRegs));
     if (warp < kMmaWarp) {
     // ------------------------------------------------------------------ decode of K and V
-    const int lr = lane >> 2, lc = lane & 3;
-    // unit u: 32 keys (u % 4) of slot number n = u / 4, which is K (n even) or V (odd) of tile n / 2
-    auto fetch = [&](int u, Codes& x, bool& live) {
-      const int n = u >> 2, k0 = (n >> 1) * kKeys + (u & 3) * 32;
+    // a lane's part of a slot: rows lr + 8 i, elements 64 half + 32 c2 .. + 32 of each
+    const int lr = (lane >> 1) & 7, c2 = lane & 1, half = lane >> 4;
+    // 16-byte chunks 4 c2 + k of a row, swizzled; 8 lanes (4 rows, both c2) hit 8 chunk positions
+    uint32_t chunk[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) chunk[k] = (uint32_t)(half * kHalf + lr * 128 + (((4 * c2 + k) ^ lr) << 4));
+    // Consecutive uses of a slot belong to different warps. A warp waits for its use by parity all the
+    // same: its own slot before lay kDecodeWarps back and waited for the release of the one kSlots
+    // before that, which (releases keep the order, but for neighbours) came after the release
+    // of the use before the last of this slot.
+    static_assert(kSlots > kDecodeWarps, "parity of the slots' uses");
+    for (int n = warp - 8; n < 2 * n_kv; n += kDecodeWarps) {  // K (n even) or V (odd) of step n / 2
+      const int k0 = (n >> 1) * kKeys;
       const int page = a.bs_log2 >= 0 ? k0 >> a.bs_log2 : k0 / a.block_size;
-      const int64_t blk = k0 < n_keys && page < a.max_blocks ? __ldg(table + page) : -1;
-      live = blk >= 0 && blk < a.num_blocks;
-      if (!live) {
-        if (k0 < n_keys) {
-          set_device_status(kStatusBadPage);
-          s_bad = 1;
+      const int64_t blk = page < a.max_blocks ? __ldg(table + page) : -1;
+      const bool live = blk >= 0 && blk < a.num_blocks;
+      uint4 codes[kKeys / 8];
+      uint32_t sc[kKeys / 8];  // two scale bytes; 0: zeros, whatever the codes
+      if (live) {
+        const int64_t r0 = (blk * a.Hkv + kvh) * a.block_size + (k0 - page * a.block_size) + lr;
+        const uint8_t* cp = ((n & 1) ? a.vc : a.kc) + r0 * kFp4RowBytes + half * 32 + c2 * 16;
+        const uint8_t* sp = ((n & 1) ? a.vs : a.ks) + r0 * kFp4ScaleBytes + half * 4 + c2 * 2;
+#pragma unroll
+        for (int i = 0; i < kKeys / 8; ++i) {
+          codes[i] = __ldg(reinterpret_cast<const uint4*>(cp + i * 8 * kFp4RowBytes));
+          sc[i] = __ldg(reinterpret_cast<const uint16_t*>(sp + i * 8 * kFp4ScaleBytes));
         }
-        return;
-      }
-      const int64_t r0 = (blk * a.Hkv + kvh) * a.block_size + (k0 - page * a.block_size) + lr;
-      const uint8_t* codes = ((n & 1) ? a.vc : a.kc) + r0 * kFp4RowBytes + lc * 16;
-      const uint8_t* scales = ((n & 1) ? a.vs : a.ks) + r0 * kFp4ScaleBytes + lc * 2;
+        if (k0 + kKeys > n_keys) {
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        x.c[i] = __ldg(reinterpret_cast<const uint4*>(codes + i * 8 * kFp4RowBytes));
-        x.s[i] = __ldg(reinterpret_cast<const uint16_t*>(scales + i * 8 * kFp4ScaleBytes));
+          for (int i = 0; i < kKeys / 8; ++i)
+            if (k0 + lr + 8 * i >= n_keys) sc[i] = 0;
+        }
+      } else {
+        set_device_status(kStatusBadPage);
+        s_bad = 1;
+#pragma unroll
+        for (int i = 0; i < kKeys / 8; ++i) {
+          codes[i] = make_uint4(0, 0, 0, 0);
+          sc[i] = 0;
+        }
       }
-    };
-    Codes cur;
-    bool cur_live = false;
-    const int total = 8 * n_kv;
-    // A warp does not write every slot, so it may skip a use of one: it waits by parity all the
-    // same, because its previous unit lay at most two slots back and waited for a release that
-    // comes after the one before last of this slot.
-    static_assert(kDecodeWarps <= 8 && kSlots > 2, "a warp's units are at most two slots apart");
-    for (int u = warp - 8; u < total; u += kDecodeWarps) {
-      fetch(u, cur, cur_live);
-      const int n = u >> 2, slot = n % kSlots;
+      const int slot = n % kSlots;
       if (!mbar_wait(&empty[slot], ((n / kSlots) & 1) ^ 1)) break;
-      unsigned char* dst = s_kv + slot * kSlotBytes + (lc >> 1) * kHalf;
+      unsigned char* dst = s_kv + slot * kSlotBytes;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        const int r = (u & 3) * 32 + lr + 8 * i;  // key of the tile
-        const int key = (n >> 1) * kKeys + r;
-        uint32_t s = cur.s[i];
-        bool zero = !cur_live || key >= n_keys;
-        if ((n & 1) && !zero) {  // V: no NaN (or infinity) reaches the product
-          if ((s & 0xFFu) >= 248u) {
-            atomicMin(&s_nan[2 * lc], key);
+      for (int i = 0; i < kKeys / 8; ++i) {
+        uint32_t s = sc[i];
+        if ((n & 1) && ((s & 0xF8u) == 0xF8u || (s & 0xF800u) == 0xF800u)) {
+          // V: no NaN (or infinity) reaches the product
+          const int key = k0 + lr + 8 * i;
+          if ((s & 0xF8u) == 0xF8u) {
+            atomicMin(&s_nan[4 * half + 2 * c2], key);
             s &= 0xFF00u;
           }
-          if ((s >> 8) >= 248u) {
-            atomicMin(&s_nan[2 * lc + 1], key);
+          if ((s & 0xF800u) == 0xF800u) {
+            atomicMin(&s_nan[4 * half + 2 * c2 + 1], key);
             s &= 0xFFu;
           }
         }
         const uint32_t f[2] = {fp4_scale_h2(s & 0xFFu), fp4_scale_h2(s >> 8)};
-        const uint32_t cw[4] = {cur.c[i].x, cur.c[i].y, cur.c[i].z, cur.c[i].w};
-        uint4 o[4];
+        const uint32_t cw[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
           uint32_t e[4];
           fp4x8_to_f16x2(cw[k], e);
-          o[k] = make_uint4(h2_mul(e[0], f[k >> 1]), h2_mul(e[1], f[k >> 1]), h2_mul(e[2], f[k >> 1]),
-                            h2_mul(e[3], f[k >> 1]));
-          if (zero) o[k] = make_uint4(0, 0, 0, 0);
-        }
-        // 16-byte chunk 4 (lc % 2) + k of the row, swizzled; lanes of the second half take the
-        // chunks in the order 2 3 0 1, so that 8 lanes always hit 8 different chunk positions
-        const bool second = lc >= 2;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-          const uint4 val = second ? o[k ^ 2] : o[k];
-          const int ch = (lc & 1) * 4 + (second ? k ^ 2 : k);
-          *reinterpret_cast<uint4*>(dst + r * 128 + ((ch ^ (r & 7)) << 4)) = val;
+          *reinterpret_cast<uint4*>(dst + chunk[k] + i * 1024) =
+              make_uint4(h2_mul(e[0], f[k >> 1]), h2_mul(e[1], f[k >> 1]), h2_mul(e[2], f[k >> 1]), h2_mul(e[3], f[k >> 1]));
         }
       }
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");  // plain stores -> the tensor core's reads
@@ -504,48 +508,63 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_fp4_kernel(const __grid_c
     role_sync();
     } else {
     // ------------------------------------------------------------------ MMA issue
-    if (lane == 0 && n_kv > 0) {
-      const uint32_t kv0 = smem_u32(s_kv), q0 = smem_u32(s_q);
-      bool ok = true;
-      auto scores = [&](int t, int n) {  // S_t = Q_t K^T, K in slot number n
-        const uint64_t dq = desc_base(q0 + t * 2 * kHalf, 16), dk = desc_base(kv0 + (n % kSlots) * kSlotBytes, 16);
+    // The whole warp walks the loop, so that descriptors and addresses stay in uniform registers, and
+    // one lane's products and commits count: issued by one thread in a divergent branch, a product took
+    // some 70 cycles to issue, more than to run.
+    const int t = warp - kMmaWarp;  // tile
+    if (t < tiles && n_kv > 0) {
+      const uint32_t lead = elect_one();
+      const uint32_t kv0 = smem_u32(s_kv);
+      const uint64_t dq = desc_base(smem_u32(s_q) + t * 2 * kQHalf, 16);
+      // slot number n is stage n % kSlots in its use n / kSlots
+      auto wait_full = [&](int stage, int use) { return mbar_wait(&full[stage], use & 1); };
+      auto scores = [&](int stage, int j) {  // S = Q K_j^T
+        const uint64_t dk = desc_base(kv0 + stage * kSlotBytes, 16);
+        const uint32_t d = tmem + t * 128 + (j & 1) * kKeys;
 #pragma unroll
-        for (int k = 0; k < 8; ++k) {
-          const uint64_t off = (uint64_t)(((k >> 2) * kHalf + (k & 3) * 32) >> 4);
-          mma_ss(tmem + t * 128, dq + off, dk + off, kIdescQK, k > 0);
-        }
-        mma_commit(&s_full[t]);
+        for (int k = 0; k < 8; ++k)  // 16 elements each
+          mma_ss(d, dq + (uint64_t)(((k >> 2) * kQHalf + (k & 3) * 32) >> 4),
+                 dk + (uint64_t)(((k >> 2) * kHalf + (k & 3) * 32) >> 4), kIdescQK, k > 0, lead);
+        mma_commit(&s_full[t][j & 1], lead);
       };
-      auto release = [&](int n) {  // nobody waits for the last slots: no arrival may outlive the CTA
-        if (n + kSlots < 2 * n_kv) mma_commit(&empty[n % kSlots]);
-      };
-      auto wait_full = [&](int n) { return mbar_wait(&full[n % kSlots], (n / kSlots) & 1); };
-      for (int t = 0; t < tiles && ok; ++t) ok = mbar_wait(&q_full[t], 0);
-      ok = ok && wait_full(0);
+      // nobody waits for the last slots: no arrival may outlive the CTA
+      const int last_release = 2 * n_kv - kSlots;
+      bool ok = mbar_wait(&q_full[t], 0) && wait_full(0, 0);
       if (ok) {
         tc_fence_after();
-        for (int t = 0; t < tiles; ++t) scores(t, 0);
-        release(0);
+        scores(0, 0);
+        if (0 < last_release) mma_commit(&empty[0], lead);
       }
+      int kst = 2 % kSlots, kuse = 0, vst = 1, vuse = 0;  // stages and uses of K_{j+1} and V_j
+      static_assert(kSlots % 2 == 0 && kSlots > 2, "K and V keep their parity of stages");
       for (int j = 0; ok && j < n_kv; ++j) {
-        const int nv = 2 * j + 1, nk = 2 * j + 2;
-        const bool more = j + 1 < n_kv;
-        ok = wait_full(nv) && (!more || wait_full(nk));
-        for (int t = 0; ok && t < tiles; ++t) {
-          ok = mbar_wait(&p_ready[t], j & 1);
+        if (j + 1 < n_kv) {
+          // S of the next step: its buffer held the weights of step j - 1, whose product was issued before
+          ok = wait_full(kst, kuse);
           if (!ok) break;
           tc_fence_after();
-          const uint64_t dv = desc_base(kv0 + (nv % kSlots) * kSlotBytes, kHalf);
-#pragma unroll
-          for (int k = 0; k < 8; ++k)  // 16 keys each
-            mma_ts(tmem + 256 + t * 128, tmem + t * 128 + 8 * k, dv + (uint64_t)((k * 2048) >> 4), kIdescPV,
-                   j > 0 || k > 0);
-          mma_commit(&pv_done[t]);
-          if (more) scores(t, nk);
+          scores(kst, j + 1);
+          if (2 * j + 2 < last_release) mma_commit(&empty[kst], lead);
+          kst += 2;
+          if (kst >= kSlots) {
+            kst -= kSlots;
+            ++kuse;
+          }
         }
-        if (ok) {
-          release(nv);
-          if (more) release(nk);
+        ok = wait_full(vst, vuse) && mbar_wait(&p_ready[t][j & 1], (j >> 1) & 1);
+        if (!ok) break;
+        tc_fence_after();
+        const uint64_t dv = desc_base(kv0 + vst * kSlotBytes, kHalf);
+        const uint32_t p = tmem + t * 128 + (j & 1) * kKeys;
+#pragma unroll
+        for (int k = 0; k < kKeys / 16; ++k)  // 16 keys each
+          mma_ts(tmem + kColO + t * kD, p + 8 * k, dv + (uint64_t)((k * 2048) >> 4), kIdescPV, j > 0 || k > 0, lead);
+        mma_commit(&pv_done[t], lead);
+        if (2 * j + 1 < last_release) mma_commit(&empty[vst], lead);
+        vst += 2;
+        if (vst >= kSlots) {
+          vst -= kSlots;
+          ++vuse;
         }
       }
     }
@@ -555,7 +574,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_fp4_kernel(const __grid_c
   }
   tc_fence_before();
   __syncthreads();
-  if (warp == kMmaWarp) {
+  if (warp == kMmaWarp + 1) {
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
   }
