@@ -96,8 +96,23 @@ def ptr(t: torch.Tensor | None) -> int | None:
     return None if t is None else t.data_ptr()
 
 
+# The current stream's handle without building a torch.cuda.Stream (0.2 instead of 2 us a call), where
+# this torch has the two functions.
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+_raw_device = getattr(torch._C, "_cuda_getDevice", None)
+
+
 def stream_ptr() -> int:
+    if _raw_stream is not None and _raw_device is not None and torch.cuda.is_initialized():
+        return _raw_stream(_raw_device())
     return torch.cuda.current_stream().cuda_stream
+
+
+def current_device() -> int:
+    """Index of the current CUDA device."""
+    if _raw_device is not None and torch.cuda.is_initialized():
+        return _raw_device()
+    return torch.cuda.current_device()
 
 
 def check(rc: int, what: str) -> None:

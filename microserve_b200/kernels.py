@@ -315,11 +315,15 @@ def fp4_cache_shapes(num_blocks: int, block_size: int, kv_heads: int, head_dim: 
 
 def _on_current_device(what: str, *tensors: torch.Tensor) -> None:
     """Every tensor on the current CUDA device, whose current stream the kernel runs on."""
-    dev = torch.cuda.current_device() if tensors[0].is_cuda else -1
+    dev = tensors[0].get_device()  # -1: not a CUDA tensor
     for t in tensors:
-        if t.get_device() != dev or dev < 0:
-            raise ValueError(f"{what}: every tensor must be on the current CUDA device (one is on {t.device}; "
-                             "use torch.cuda.device(...))")
+        if t.get_device() != dev:
+            break
+    else:
+        if dev >= 0 and dev == _lib.current_device():
+            return
+    raise ValueError(f"{what}: every tensor must be on the current CUDA device, these are on "
+                     f"{sorted({str(t.device) for t in tensors})} (use torch.cuda.device(...))")
 
 
 def _fp4_cache(what: str, k_cache, v_cache, k_scale, v_scale, head_dim: int) -> tuple[int, int, int]:
@@ -327,12 +331,15 @@ def _fp4_cache(what: str, k_cache, v_cache, k_scale, v_scale, head_dim: int) -> 
     NB, Hkv, BS, half = shape = k_cache.shape
     if half * 2 != head_dim:
         raise ValueError(f"{what}: head_dim {head_dim} does not match a cache of {half} code bytes a row")
-    if v_cache.shape != shape or k_scale.shape != v_scale.shape or k_scale.shape != (NB, Hkv, BS, half // 8):
+    scales = k_scale.shape
+    if v_cache.shape != shape or v_scale.shape != scales or scales != (NB, Hkv, BS, half // 8):
         raise ValueError(f"{what}: cache shapes {tuple(shape)} {tuple(v_cache.shape)} {tuple(k_scale.shape)} "
                          f"{tuple(v_scale.shape)} do not belong together")
-    for t in (k_cache, v_cache, k_scale, v_scale):
-        if t.dtype is not torch.uint8 or not t.is_contiguous():
-            raise ValueError(f"{what}: the 4-bit cache is contiguous uint8")
+    u8 = torch.uint8
+    if not (k_cache.dtype is u8 and v_cache.dtype is u8 and k_scale.dtype is u8 and v_scale.dtype is u8
+            and k_cache.is_contiguous() and v_cache.is_contiguous() and k_scale.is_contiguous()
+            and v_scale.is_contiguous()):
+        raise ValueError(f"{what}: the 4-bit cache is contiguous uint8")
     return NB, Hkv, BS
 
 
@@ -374,8 +381,7 @@ def load_kv_fp4(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Ten
         raise ValueError("load_kv_fp4: slot_mapping must be contiguous int64 [T]")
     _on_current_device("load_kv_fp4", k_cache, v_cache, k_scale, v_scale, slot_mapping)
     T = slot_mapping.shape[0]
-    k = torch.empty((T, Hkv, 128), dtype=torch.float16, device=k_cache.device)
-    v = torch.empty_like(k)
+    k, v = k_cache.new_empty((2, T, Hkv, 128), dtype=torch.float16).unbind(0)
     check(_lib.load().ms_load_kv_fp4(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                                      NB, BS, T, Hkv, 128, slot_mapping.data_ptr(), k.data_ptr(), v.data_ptr(),
                                      stream_ptr()), "ms_load_kv_fp4")
@@ -388,7 +394,7 @@ def _fp4_query(what: str, query: torch.Tensor,
     if query.dtype is not torch.float16 or query.dim() != 3:
         raise ValueError(f"{what}: query must be fp16 [tokens, heads, head_dim]")
     if out is None:
-        out = torch.empty(query.shape, dtype=torch.float16, device=query.device)
+        out = torch.empty_like(query, memory_format=torch.contiguous_format)
     elif out.shape != query.shape or out.dtype is not torch.float16 or not out.is_contiguous():
         raise ValueError(f"{what}: out must be contiguous fp16 of query's shape")
     elif out.data_ptr() % 16 != 0:
@@ -401,10 +407,14 @@ def _fp4_query(what: str, query: torch.Tensor,
 
 
 def _int32(what: str, name: str, t: torch.Tensor, *shape: int) -> None:
-    if t.dtype is not torch.int32 or not t.is_contiguous() or t.dim() != len(shape) \
-            or any(s >= 0 and s != n for s, n in zip(shape, t.shape)):
-        raise ValueError(f"{what}: {name} must be contiguous int32 of shape "
-                         f"[{', '.join('*' if s < 0 else str(s) for s in shape)}]")
+    if t.dtype is torch.int32 and t.is_contiguous() and t.dim() == len(shape):
+        for s, n in zip(shape, t.shape):
+            if s >= 0 and s != n:
+                break
+        else:
+            return
+    raise ValueError(f"{what}: {name} must be contiguous int32 of shape "
+                     f"[{', '.join('*' if s < 0 else str(s) for s in shape)}]")
 
 
 def paged_decode_fp4(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
