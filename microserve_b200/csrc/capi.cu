@@ -317,7 +317,8 @@ int ms_store_kv_fp4(const void* k, const void* v, int64_t k_token_stride, int64_
                     int64_t v_token_stride, int64_t v_head_stride, int64_t T, int kv_heads, int head_dim,
                     const int64_t* slots, void* k_cache, void* v_cache, void* k_scale, void* v_scale,
                     int64_t num_blocks, int block_size, void* stream) {
-  if (T < 0 || T > INT32_MAX) return fail(MS_ERR_INVALID, "ms_store_kv_fp4: bad sizes T=%lld", (long long)T);
+  if (T < 0 || T > INT32_MAX || kv_heads > 65535)
+    return fail(MS_ERR_INVALID, "ms_store_kv_fp4: bad sizes T=%lld kv_heads=%d", (long long)T, kv_heads);
   const int rc = check_fp4_cache("ms_store_kv_fp4", k_cache, v_cache, k_scale, v_scale, num_blocks, kv_heads,
                                  head_dim, block_size);
   if (rc != MS_OK || T == 0) return rc;
@@ -335,7 +336,8 @@ int ms_store_kv_fp4(const void* k, const void* v, int64_t k_token_stride, int64_
 int ms_load_kv_fp4(const void* k_cache, const void* v_cache, const void* k_scale, const void* v_scale,
                    int64_t num_blocks, int block_size, int64_t T, int kv_heads, int head_dim, const int64_t* slots,
                    void* k, void* v, void* stream) {
-  if (T < 0 || T > INT32_MAX) return fail(MS_ERR_INVALID, "ms_load_kv_fp4: bad sizes T=%lld", (long long)T);
+  if (T < 0 || T > INT32_MAX || kv_heads > 65535)
+    return fail(MS_ERR_INVALID, "ms_load_kv_fp4: bad sizes T=%lld kv_heads=%d", (long long)T, kv_heads);
   const int rc = check_fp4_cache("ms_load_kv_fp4", k_cache, v_cache, k_scale, v_scale, num_blocks, kv_heads, head_dim,
                                  block_size);
   if (rc != MS_OK || T == 0) return rc;

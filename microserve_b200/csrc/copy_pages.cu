@@ -86,6 +86,10 @@ cudaError_t launch_copy_pages(void* cache, int64_t cache_plane_stride, int row_b
                               int64_t num_pages, const int32_t* src, const int32_t* dst, const int32_t* tokens, int n,
                               int num_sms, cudaStream_t stream) {
   if (n == 0 || planes == 0) return cudaSuccess;
+  if (tokens == nullptr) {  // whole pages: one run each (64 pages x 36 layers, 4-bit: 212 us, in runs 247)
+    block_size *= outer;
+    outer = 1;
+  }
   CopyArgs a = {};
   a.src = src;
   a.dst = dst;

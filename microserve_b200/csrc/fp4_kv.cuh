@@ -54,48 +54,80 @@ __device__ __forceinline__ uint32_t h2_mul(uint32_t a, uint32_t b) {
 // Scale byte in both halves of an f16x2.
 __device__ __forceinline__ uint32_t fp4_scale_h2(uint32_t byte) { return byte * 0x00800080u; }
 
-// Scale byte of a group whose largest |x| has the fp16 bits `amax` (0..0x7FFF).
-__device__ __forceinline__ uint32_t fp4_scale_code(uint32_t amax) {
-  if (amax > 0x7C00u) return kFp4NanScaleCode;
-  const float a = fminf(__half2float(__ushort_as_half((unsigned short)amax)), 65504.f);
-  const float v = __fdiv_rn(a, 6.f);
-  uint32_t code;
-  if (v < 6.103515625e-05f) {  // below 2^-14: steps of 2^-17
-    code = (uint32_t)__float2int_rn(v * 131072.f);
-  } else {  // keep 3 mantissa bits, ties to even; rebias 127 -> 15
-    uint32_t b = __float_as_uint(v);
-    b += 0x7FFFFu + ((b >> 20) & 1u);
-    code = (b >> 20) - ((127u - 15u) << 3);
-  }
-  return min(code, (uint32_t)kFp4MaxScaleCode);
+// Pairs of floats in one 64-bit register: one instruction for two.
+__device__ __forceinline__ uint64_t f32x2(float x, float y) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
+  return r;
+}
+__device__ __forceinline__ void unpack2(uint64_t v, float& x, float& y) {
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
+  return r;
+}
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
+  return r;
 }
 
-// Codes of 8 fp16 elements (4 words) under scale byte `sc`, packed in one word.
-// x / s is taken as q0 = x * (1/s) and one correction by the remainder x - q0 s: exact
-// where x / s is a rounding boundary (the only place where the last bit matters).
-__device__ __forceinline__ uint32_t fp4_encode8(const uint32_t (&h)[4], uint32_t sc) {
-  if (sc == (uint32_t)kFp4NanScaleCode) return 0u;
+// Scale byte of a group whose largest |x| has the fp16 bits `amax` (0..0x7FFF).
+// a / 6 is taken as a * h + a * l with h + l = 1/6 to 48 bits: exact where it is a rounding
+// boundary (5 bits), right to 2^-24 elsewhere.
+__device__ __forceinline__ uint32_t fp4_scale_code(uint32_t amax) {
+  constexpr float kSixthHi = 1.f / 6.f, kSixthLo = (float)(1.0 / 6.0 - (double)kSixthHi);
+  const float a = __half2float(__ushort_as_half((unsigned short)min(amax, 0x7BFFu)));
+  const float v = __fmaf_rn(a, kSixthHi, __fmul_rn(a, kSixthLo));
+  // keep 3 mantissa bits, ties to even; rebias 127 -> 15
+  uint32_t b = __float_as_uint(v);
+  b += 0x7FFFFu + ((b >> 20) & 1u);
+  const uint32_t normal = (b >> 20) - ((127u - 15u) << 3);
+  const uint32_t tiny = (uint32_t)__float2int_rn(v * 131072.f);  // below 2^-14: steps of 2^-17
+  const uint32_t code = min(v < 6.103515625e-05f ? tiny : normal, (uint32_t)kFp4MaxScaleCode);
+  return amax > 0x7C00u ? (uint32_t)kFp4NanScaleCode : code;
+}
+
+// Codes of 8 fp16 elements (4 words) under scale byte `sc`, packed in one word; amax as above.
+// x / s is taken as x * h + x * l with h + l = 1 / s to 48 bits: exact where it is a rounding
+// boundary (the only place where the last bit matters).
+__device__ __forceinline__ uint32_t fp4_encode8(const uint32_t (&x)[4], uint32_t sc, uint32_t amax) {
+  uint32_t h[4] = {x[0], x[1], x[2], x[3]};
+  if (amax >= 0x7C00u) {  // rare
+    if (amax > 0x7C00u) return 0u;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // an infinity counts as the largest number
+      if ((h[i] & 0x7FFFu) == 0x7C00u) h[i] -= 1u;
+      if ((h[i] & 0x7FFF0000u) == 0x7C000000u) h[i] -= 0x10000u;
+    }
+  }
   const float s = __half2float(__ushort_as_half((unsigned short)(sc << 7)));
   const float r = sc == 0 ? 0.f : __frcp_rn(s);
-  uint32_t w = 0;
+  const float rl = __fmul_rn(__fmaf_rn(-r, s, 1.f), r);
+  const uint64_t r2 = f32x2(r, r), l2 = f32x2(rl, rl);
+  uint32_t b[4];
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     __half2 p;
     memcpy(&p, &h[i], 4);
-    float2 f = __half22float2(p);
-    f.x = fminf(fmaxf(f.x, -65504.f), 65504.f);
-    f.y = fminf(fmaxf(f.y, -65504.f), 65504.f);
-    const float qx = __fmul_rn(f.x, r), qy = __fmul_rn(f.y, r);
-    // the sign of a zero (or of a quotient that rounds to zero) is x's
-    const float cx = copysignf(__fmaf_rn(__fmaf_rn(-qx, s, f.x), r, qx), f.x);
-    const float cy = copysignf(__fmaf_rn(__fmaf_rn(-qy, s, f.y), r, qy), f.y);
-    uint32_t b;
+    const float2 f = __half22float2(p);
+    const uint64_t f2 = f32x2(f.x, f.y);
+    float qx, qy;
+    unpack2(fma2(f2, r2, mul2(f2, l2)), qx, qy);
+    qx = copysignf(qx, f.x);  // the sign of a zero is x's
+    qy = copysignf(qy, f.y);
     asm("{\n\t.reg .b8 t;\n\tcvt.rn.satfinite.e2m1x2.f32 t, %1, %2;\n\tcvt.u32.u8 %0, t;\n\t}"
-        : "=r"(b)
-        : "f"(cy), "f"(cx));
-    w |= b << (8 * i);
+        : "=r"(b[i])
+        : "f"(qy), "f"(qx));
   }
-  return w;
+  return prmt(prmt(b[0], b[1], 0x0040u), prmt(b[2], b[3], 0x0040u), 0x5410u);
 }
 
 }  // namespace ms

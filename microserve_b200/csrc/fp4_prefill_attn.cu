@@ -162,26 +162,6 @@ __device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&v)[16]) {
       : "r"(addr));
 }
 
-// Pairs of floats in one 64-bit register: one instruction for two.
-__device__ __forceinline__ uint64_t f32x2(float x, float y) {
-  uint64_t r;
-  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(x), "f"(y));
-  return r;
-}
-__device__ __forceinline__ void unpack2(uint64_t v, float& x, float& y) {
-  asm("mov.b64 {%0, %1}, %2;" : "=f"(x), "=f"(y) : "l"(v));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-  uint64_t r;
-  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(a), "l"(b), "l"(c));
-  return r;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
-  return r;
-}
-
 struct PrefillArgs {
   const __half* q;  // [T, Hq, D], token stride q_ts elements
   int64_t q_ts;
