@@ -239,12 +239,15 @@ int ms_paged_decode_fp4(const void* q, int64_t q_token_stride, const void* k_cac
 /* ms_paged_prefill_fp8 over the 4-bit cache, any Hq / Hkv <= 8, softmax_scale > 0: sequence s has queries
  * q[cu_q[s] .. cu_q[s+1]) at positions kv_lens[s] - q_len_s + i, each seeing the keys
  * up to its own position (none below position 0: output 0). Rows of out behind
- * cu_q[num_seqs] are not written. */
+ * cu_q[num_seqs] are not written, offsets outside [0, total_q] are cut. Workspace as for
+ * ms_paged_decode_fp4. */
+size_t ms_paged_prefill_fp4_workspace_size(int num_seqs, int64_t total_q, int Hq, int Hkv, int max_blocks,
+                                           int block_size);
 int ms_paged_prefill_fp4(const void* q, int64_t q_token_stride, const void* k_cache, const void* v_cache,
                          const void* k_scale, const void* v_scale, int64_t num_blocks, const int32_t* block_tables,
                          const int32_t* cu_q, const int32_t* kv_lens, void* out, int num_seqs, int64_t total_q,
                          int Hq, int Hkv, int head_dim, int block_size, int max_blocks, float softmax_scale,
-                         void* stream);
+                         void* workspace, size_t workspace_bytes, void* stream);
 
 /* Page copies inside a paged cache (fork of a sequence, moves), all planes (K and V of
  * every layer), codes and scales in one launch: for i < n, tokens [0, tokens[i]) (null:

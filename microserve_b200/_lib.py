@@ -60,7 +60,8 @@ SIGNATURES: dict[str, tuple] = {
                                   sz, vp]),
     "ms_paged_decode_fp4_workspace_size": (sz, [i32, i32, i32, i32, i32]),
     "ms_paged_prefill_fp4": (i32, [vp, i64, vp, vp, vp, vp, i64, vp, vp, vp, vp, i32, i64, i32, i32, i32, i32, i32,
-                                   f32, vp]),
+                                   f32, vp, sz, vp]),
+    "ms_paged_prefill_fp4_workspace_size": (sz, [i32, i64, i32, i32, i32, i32]),
     "ms_copy_pages": (i32, [vp, i64, i32, vp, i64, i32, i32, i32, i32, i64, vp, vp, vp, i32, vp]),
     "ms_varlen_prefill": (i32, [vp, vp, vp, vp, vp, i32, i64, i32, i32, i32, f32, vp]),
 }

@@ -1,7 +1,7 @@
 """Build the in-tree CUDA library `libmicroserve_b200.so` for sm_100a.
 
 Each `csrc/*.cu` is compiled with nvcc as relocatable device code (the
-kernels share one device status word; WHOLE_PROGRAM names the exceptions), then device-linked into a shared
+kernels share one device status word), then device-linked into a shared
 library next to this file. Objects go to `_build/` at the repository root.
 Rebuilds only what changed (source or header newer than its object).
 """
@@ -20,10 +20,7 @@ BUILD = ROOT / "_build"
 LIB = PKG / "libmicroserve_b200.so"
 
 ARCH = ["-gencode", "arch=compute_100a,code=sm_100a"]
-# Files compiled as whole programs (no relocatable device code): setmaxnreg is ignored otherwise.
-# They define MS_WHOLE_PROGRAM (common.cuh).
-WHOLE_PROGRAM = {"fp4_prefill_attn"}
-FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC,-O2",
+FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-rdc=true", "-Xcompiler", "-fPIC,-O2",
          "--expt-relaxed-constexpr", "-I", str(ROOT / "include")]
 
 
@@ -49,8 +46,7 @@ def build(verbose: bool = False, extra_flags: list[str] | None = None) -> Path:
     for s in srcs:
         o = BUILD / (s.stem + ".o")
         if _stale(o, s, headers):
-            own = ["-rdc=false"] if s.stem in WHOLE_PROGRAM else ["-rdc=true"]
-            jobs.append([nvcc, *ARCH, *flags, *own, "-c", str(s), "-o", str(o)])
+            jobs.append([nvcc, *ARCH, *flags, "-c", str(s), "-o", str(o)])
 
     def run(cmd):
         if verbose:

@@ -102,10 +102,8 @@ int ms_get_device_status(int* status, void* stream) {
                                             S(stream));
   if (e == cudaSuccess)
     e = cudaMemcpyToSymbolAsync(ms::g_device_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, S(stream));
-  int own = 0;
-  if (e == cudaSuccess) e = ms::prefill_fp4_take_status(&own, S(stream));
   if (e == cudaSuccess) e = cudaStreamSynchronize(S(stream));
-  *status = host != 0 ? host : own;
+  *status = host;
   return check_cuda(e, "ms_get_device_status");
 }
 
@@ -375,11 +373,19 @@ int ms_paged_decode_fp4(const void* q, int64_t q_token_stride, const void* k_cac
                     "ms_paged_decode_fp4");
 }
 
+size_t ms_paged_prefill_fp4_workspace_size(int num_seqs, int64_t total_q, int Hq, int Hkv, int max_blocks,
+                                           int block_size) {
+  if (num_seqs <= 0 || total_q <= 0 || total_q > INT32_MAX || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 ||
+      Hq / Hkv > 8 || max_blocks <= 0 || block_size <= 0)
+    return 0;
+  return ms::prefill_fp4_workspace_bytes(num_seqs, (int)total_q, Hq, Hkv, max_blocks, block_size, num_sms());
+}
+
 int ms_paged_prefill_fp4(const void* q, int64_t q_token_stride, const void* k_cache, const void* v_cache,
                          const void* k_scale, const void* v_scale, int64_t num_blocks, const int32_t* block_tables,
                          const int32_t* cu_q, const int32_t* kv_lens, void* out, int num_seqs, int64_t total_q,
                          int Hq, int Hkv, int head_dim, int block_size, int max_blocks, float softmax_scale,
-                         void* stream) {
+                         void* workspace, size_t workspace_bytes, void* stream) {
   if (num_seqs < 0 || total_q < 0 || max_blocks <= 0 || total_q > INT32_MAX)
     return fail(MS_ERR_INVALID, "ms_paged_prefill_fp4: bad sizes");
   int rc = check_fp4_cache("ms_paged_prefill_fp4", k_cache, v_cache, k_scale, v_scale, num_blocks, Hkv, head_dim,
@@ -389,9 +395,14 @@ int ms_paged_prefill_fp4(const void* q, int64_t q_token_stride, const void* k_ca
   rc = check_fp4_query("ms_paged_prefill_fp4", q, q_token_stride, out, Hq, Hkv, softmax_scale);
   if (rc != MS_OK) return rc;
   if (!block_tables || !cu_q || !kv_lens) return fail(MS_ERR_INVALID, "ms_paged_prefill_fp4: null pointer");
+  const size_t need =
+      ms::prefill_fp4_workspace_bytes(num_seqs, (int)total_q, Hq, Hkv, max_blocks, block_size, num_sms());
+  if (workspace_bytes < need || workspace == nullptr)
+    return fail(MS_ERR_WORKSPACE, "ms_paged_prefill_fp4: workspace %zu < %zu bytes", workspace_bytes, need);
+  if (!aligned16(workspace)) return fail(MS_ERR_INVALID, "ms_paged_prefill_fp4: workspace not 16-byte aligned");
   return check_cuda(ms::launch_prefill_fp4(q, q_token_stride, k_cache, v_cache, k_scale, v_scale, num_blocks,
                                            block_tables, cu_q, kv_lens, out, num_seqs, (int)total_q, Hq, Hkv,
-                                           block_size, max_blocks, softmax_scale, S(stream)),
+                                           block_size, max_blocks, softmax_scale, workspace, num_sms(), S(stream)),
                     "ms_paged_prefill_fp4");
 }
 
@@ -584,9 +595,7 @@ int ms_fp8_gemm_rowpar_ar_rmsnorm(const void* xq, const float* sx, const void* w
 int ms_set_wait_limit(uint64_t ns) {
   if (ns == 0) return fail(MS_ERR_INVALID, "ms_set_wait_limit: limit must be > 0");
   const unsigned long long v = ns;
-  cudaError_t e = cudaMemcpyToSymbol(ms::g_wait_limit_ns, &v, sizeof(v));
-  if (e == cudaSuccess) e = ms::prefill_fp4_set_wait_limit(v);
-  return check_cuda(e, "ms_set_wait_limit");
+  return check_cuda(cudaMemcpyToSymbol(ms::g_wait_limit_ns, &v, sizeof(v)), "ms_set_wait_limit");
 }
 
 int ms_row_amax(const void* x, int64_t ldx, int64_t M, int64_t K, float* amax, void* stream) {

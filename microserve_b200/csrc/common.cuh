@@ -37,14 +37,7 @@ enum DeviceStatus : int {
   kStatusBadPage = 3,  // a slot, page or length outside the cache was skipped (4-bit cache, page copies)
 };
 
-// A file that defines MS_WHOLE_PROGRAM is compiled without relocatable device code (build.py),
-// which setmaxnreg needs, and keeps a status word and a wait limit of its own; the entry points
-// that read and set them know of both.
-#ifdef MS_WHOLE_PROGRAM
-static __device__ int g_device_status = 0;
-#else
 extern __device__ int g_device_status;
-#endif
 
 // Host-side count of kernel launches issued by the library (for launch
 // accounting in benchmarks; a CUDA-graph replay re-runs captured launches
@@ -227,11 +220,7 @@ __device__ __forceinline__ uint64_t global_ns() {
 // waits last microseconds to milliseconds; the limit only ends a wait whose
 // event can no longer come (a peer that died or never joined). Default 4 s.
 constexpr uint64_t kDefaultWaitLimitNs = 4000000000ull;
-#ifdef MS_WHOLE_PROGRAM
-static __device__ unsigned long long g_wait_limit_ns = kDefaultWaitLimitNs;
-#else
 extern __device__ unsigned long long g_wait_limit_ns;
-#endif
 
 __device__ __forceinline__ uint64_t wait_limit_ns() {
   return *static_cast<volatile unsigned long long*>(&g_wait_limit_ns);

@@ -3,9 +3,12 @@
 // kv_lens[s] - q_len + i, each attending to the cached keys up to its own position.
 //
 // Tensor bound (4 * 128 * Hq operations per visible pair), so both products run on tcgen05
-// with fp32 accumulators in TMEM. One CTA handles two tiles of 128 query rows, a row being
-// a (token, query head) pair of the G = Hq / Hkv heads that share a kv head, over steps of
-// 64 keys that both read:
+// with fp32 accumulators in TMEM. An item is two tiles of 128 query rows of one kv head, a row
+// being a (token, query head) pair of the G = Hq / Hkv heads that share it, over steps of 64
+// keys that both tiles read. The steps of all items (sequence, block of tokens, kv head) form
+// one list that is dealt evenly to one CTA per SM, whatever the lengths are; an item that
+// crosses CTAs leaves fp32 partials (O, reference, sum) in the workspace, joined by a second kernel.
+// The roles below walk a CTA's items on their own, so decoding runs ahead into the next one.
 //   warps 0-3, 4-7   softmax of tile 0 / 1: a thread owns a row. It reads its 64 scores of a
 //                    step from TMEM, writes the weights over them as f16, and keeps the row's
 //                    maximum and sum (fp32).
@@ -26,10 +29,10 @@
 // more. Weights are rounded to f16 for the second product (2^-11 relative; the first
 // rounding below fp32 in the kernel, K and V are exact), the row sums take them unrounded.
 //
-// V rows behind the sequence's end and rows of bad pages are written as zeros, and a NaN group
-// of V as zeros too, because a zero weight does not hide a NaN from the product: the first
-// key with a NaN is kept per 16 elements, and the rows that see it get NaN at the end.
-#define MS_WHOLE_PROGRAM  // setmaxnreg below
+// V rows behind an item's last key and rows of bad pages are written as zeros, and a NaN group
+// of V as zeros too, because a zero weight does not hide a NaN from the product; where one was
+// met, the first key with a NaN is looked up per 16 elements at the end of the item, and the rows
+// that see it get NaN.
 #include <mutex>
 
 #include "fp4_kv.cuh"
@@ -150,9 +153,6 @@ __device__ __forceinline__ float max32(const float (&x)[32], float m) {
   return fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
 }
 
-// Every thread of the CTA, from the ends of the roles.
-__device__ __forceinline__ void role_sync() { asm volatile("bar.sync 1, %0;" ::"n"(kThreads) : "memory"); }
-
 __device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&v)[16]) {
   uint32_t* r = reinterpret_cast<uint32_t*>(v);
   asm volatile(
@@ -160,6 +160,16 @@ __device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&v)[16]) {
       : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]),
         "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
       : "r"(addr));
+}
+
+__device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool in) {  // not in: zeros
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+
+// mbar_wait by a whole warp, with one answer (lanes may run out of time at different moments).
+__device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t phase) {
+  return __all_sync(0xffffffffu, mbar_wait(bar, phase)) != 0;
 }
 
 struct PrefillArgs {
@@ -170,23 +180,194 @@ struct PrefillArgs {
   const int32_t* tables;  // [S, max_blocks]
   const int32_t* cu_q;    // [S + 1]
   const int32_t* kv_lens;
-  __half* out;  // [T, Hq, D]
-  int num_seqs, total_q, Hkv, G, block_size, bs_log2, max_blocks;
+  __half* out;       // [T, Hq, D]
+  int4* open_items;  // workspace: per CTA, the item that it leaves open: CTAs it goes on in, seq, block, kv head
+  float* ws;         // workspace: [CTAs][2] partials of kPartFloats
+  int num_seqs, total_q, Hkv, G, tok, block_size, bs_log2, max_blocks;  // tok: query tokens of an item, 2 (128 / G)
+  int inv_g;  // r / G = r * inv_g >> 16 for rows r of a tile
   int cap;  // tokens that a table row can hold
   float scale_log2;
 };
 
-struct Item {
-  int seq, tok0;  // first query token of the CTA within its sequence
+// The list is dealt in units of a step's time; an item's change of Q, output or partial and first scores, in which the
+// tensor core idles, count as kItemUnits more in front of its steps.
+constexpr int kItemUnits = 4;
+constexpr int kMinShare = 8;  // units of a CTA at least
+constexpr int kPartRows = 2 * kRows;
+constexpr int kPartFloats = kPartRows * (kD + 2);  // O as [32 x 4 elements][row][4], then (reference, sum) per row
+
+struct Seq {
+  int q_start, q_len, kv_len, prefix, blocks;  // prefix: position of the first query
 };
+__device__ __forceinline__ Seq seq_of(const PrefillArgs& a, int s) {
+  Seq q;
+  q.q_start = min(max(a.cu_q[s], 0), a.total_q);
+  q.q_len = max(min(a.cu_q[s + 1], a.total_q) - q.q_start, 0);
+  const int kv = a.kv_lens[s];
+  q.prefix = kv - q.q_len;
+  q.kv_len = min(kv, a.cap);
+  q.blocks = (q.q_len + a.tok - 1) / a.tok;
+  return q;
+}
+// Keys that block b of a sequence sees, and its steps (one even without keys: its rows become zeros).
+__device__ __forceinline__ int keys_of(const PrefillArgs& a, const Seq& q, int b) {
+  return max(0, min(q.kv_len, q.prefix + min((b + 1) * a.tok, q.q_len)));
+}
+__device__ __forceinline__ int steps_of(int keys) { return max(1, (keys + kKeys - 1) / kKeys); }
+
+// Place in the CTA's list: item (s, b, h) of `steps` steps begins at unit `start` of the CTA's `count` (negative: in an
+// earlier CTA). [j0, j1): its steps of this CTA, none if only units in front of them are; j0 is the CTA's step `first`.
+struct Cursor {
+  int s, b, h, steps, keys, start, j0, j1, first;
+  Seq q;
+  __device__ __forceinline__ void own_steps(int count) {
+    j0 = max(0, -start - kItemUnits);
+    j1 = max(j0, min(steps, count - start - kItemUnits));
+  }
+  __device__ __forceinline__ int end() const { return start + kItemUnits + steps; }
+  // to the next item with steps of this CTA; false: there is none
+  __device__ __forceinline__ bool next_item(const PrefillArgs& a, int count) {
+    start = end();
+    first += j1 - j0;
+    if (start + kItemUnits >= count) return false;
+    if (++h == a.Hkv) {
+      h = 0;
+      ++b;
+      while (b >= q.blocks) {
+        b = 0;
+        if (++s >= a.num_seqs) return false;  // only if the lengths changed meanwhile
+        q = seq_of(a, s);
+      }
+      keys = keys_of(a, q, b);
+      steps = steps_of(keys);
+    }
+    own_steps(count);
+    return true;
+  }
+};
+
+// The 16-element groups in which V has a NaN among keys [k0, k1) up to `lim` of the calling lane's row, a
+// bit each. A warp; rare, so it simply reads the scales again.
+__device__ __noinline__ uint32_t nan_groups(const PrefillArgs& a, int seq, int kvh, int k0, int k1, int lim) {
+  int first[8];
+#pragma unroll
+  for (int g = 0; g < 8; ++g) first[g] = INT32_MAX;
+  for (int k = k0 + (int)(threadIdx.x & 31); k < k1; k += 32) {
+    const int pg = k / a.block_size;
+    const int64_t blk = pg < a.max_blocks ? a.tables[(int64_t)seq * a.max_blocks + pg] : -1;
+    if (blk < 0 || blk >= a.num_blocks) continue;
+    const uint8_t* sp = a.vs + ((blk * a.Hkv + kvh) * a.block_size + (k - pg * a.block_size)) * kFp4ScaleBytes;
+#pragma unroll
+    for (int g = 0; g < 8; ++g)
+      if (sp[g] >= 248) first[g] = min(first[g], k);
+  }
+  __syncwarp();
+  uint32_t bits = 0;
+#pragma unroll
+  for (int g = 0; g < 8; ++g) bits |= __reduce_min_sync(0xffffffffu, first[g]) <= lim ? 1u << g : 0u;
+  return bits;
+}
+
+__device__ __forceinline__ int warp_scan(int v) {  // inclusive
+  const int lane = threadIdx.x & 31;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int up = __shfl_up_sync(0xffffffffu, v, o);
+    if (lane >= o) v += up;
+  }
+  return v;
+}
+
+// Units of one kv head in sequence s0 + lane (a whole warp: long sequences are shared by its lanes).
+__device__ __forceinline__ int seq_units(const PrefillArgs& a, int s0) {
+  const int lane = threadIdx.x & 31;
+  const bool in = s0 + lane < a.num_seqs;
+  const Seq q = in ? seq_of(a, s0 + lane) : Seq{0, 0, 0, 0, 0};
+  if (in && q.kv_len < a.kv_lens[s0 + lane]) set_device_status(kStatusBadPage);
+  int mine = 0;
+  constexpr int kOwn = 4;
+  if (q.blocks <= kOwn)
+    for (int b = 0; b < q.blocks; ++b) mine += kItemUnits + steps_of(keys_of(a, q, b));
+  uint32_t longer = __ballot_sync(0xffffffffu, q.blocks > kOwn);
+  while (longer != 0) {
+    const int l = __ffs(longer) - 1;
+    longer &= longer - 1;
+    const Seq o{0, __shfl_sync(0xffffffffu, q.q_len, l), __shfl_sync(0xffffffffu, q.kv_len, l),
+                __shfl_sync(0xffffffffu, q.prefix, l), __shfl_sync(0xffffffffu, q.blocks, l)};
+    int part = 0;
+    for (int b = lane; b < o.blocks; b += 32) part += kItemUnits + steps_of(keys_of(a, o, b));
+    part = __shfl_sync(0xffffffffu, warp_scan(part), 31);
+    if (lane == l) mine = part;
+  }
+  return mine;
+}
+
+// This CTA's share of the list: its units (0: no steps), its first item, and the share of every CTA. A warp.
+__device__ __forceinline__ int find_share(const PrefillArgs& a, Cursor& c, int64_t& share) {
+  const int lane = threadIdx.x & 31;
+  int64_t total = 0;
+  int last = 0;  // this lane's sequence of the last 32
+  for (int s0 = 0; s0 < a.num_seqs; s0 += 32) {
+    last = seq_units(a, s0);
+    total += (int64_t)__shfl_sync(0xffffffffu, warp_scan(last), 31) * a.Hkv;
+  }
+  const int64_t even = (total + gridDim.x - 1) / gridDim.x;
+  share = even > kMinShare ? even : kMinShare;
+  const int64_t begin = (int64_t)blockIdx.x * share;
+  if (begin >= total) return 0;
+  int64_t at = 0;  // units before sequence s0
+  int s0 = 0;
+  for (;; s0 += 32) {
+    if (s0 >= a.num_seqs) return 0;  // only if the lengths changed meanwhile
+    const int mine = a.num_seqs <= 32 ? last : seq_units(a, s0);
+    const int inc = warp_scan(mine);
+    const int64_t end = at + (int64_t)inc * a.Hkv;
+    const uint32_t hit = __ballot_sync(0xffffffffu, begin < end);
+    if (hit == 0) {
+      at = __shfl_sync(0xffffffffu, end, 31);
+      continue;
+    }
+    const int l = __ffs(hit) - 1;
+    at += (int64_t)__shfl_sync(0xffffffffu, inc - mine, l) * a.Hkv;
+    c.s = s0 + l;
+    break;
+  }
+  if (c.s >= a.num_seqs) return 0;
+  c.q = seq_of(a, c.s);
+  for (int b0 = 0;; b0 += 32) {
+    const int keys = b0 + lane < c.q.blocks ? keys_of(a, c.q, b0 + lane) : 0;
+    const int mine = b0 + lane < c.q.blocks ? kItemUnits + steps_of(keys) : 0;
+    const int inc = warp_scan(mine);
+    const uint32_t hit = __ballot_sync(0xffffffffu, begin < at + (int64_t)inc * a.Hkv);
+    if (hit == 0) {
+      if (b0 + 32 >= c.q.blocks) return 0;  // as above
+      at += (int64_t)__shfl_sync(0xffffffffu, inc, 31) * a.Hkv;
+      continue;
+    }
+    const int l = __ffs(hit) - 1;
+    at += (int64_t)__shfl_sync(0xffffffffu, inc - mine, l) * a.Hkv;
+    c.b = b0 + l;
+    c.steps = max(__shfl_sync(0xffffffffu, mine, l) - kItemUnits, 1);
+    c.keys = __shfl_sync(0xffffffffu, keys, l);
+    break;
+  }
+  const int off = (int)(begin - at), units = kItemUnits + c.steps;
+  c.h = off / units;
+  c.start = -(off - c.h * units);
+  const int count = (int)(total - begin < share ? total - begin : share);
+  c.own_steps(count);
+  return c.j0 < c.j1 || c.next_item(a, count) ? count : 0;
+}
 
 __global__ void __launch_bounds__(kThreads, 1) prefill_fp4_kernel(const __grid_constant__ PrefillArgs a) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
-  __shared__ uint64_t q_full[2], full[kSlots], empty[kSlots], s_full[2][2], p_ready[2][2], pv_done[2];
+  __shared__ uint64_t q_full[2], full[kSlots], empty[kSlots], s_full[2][2], p_ready[2][2], pv_done[2][2];
   __shared__ uint32_t s_tmem;
-  __shared__ Item s_item;
-  __shared__ int s_nan[8];  // first key whose V group is NaN, per 16 elements
-  __shared__ int s_bad;     // the sequence has a page outside the cache
+  __shared__ Cursor s_first;
+  __shared__ int s_count;
+  __shared__ int64_t s_share;
+  __shared__ int s_seen_nan;  // a V group with a NaN was decoded
+  __shared__ int s_bad;       // a page outside the cache was met
   unsigned char* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   unsigned char* s_q = smem;
   unsigned char* s_kv = smem + kQBytes;
@@ -194,50 +375,36 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_fp4_kernel(const __grid_c
   pdl_wait();
   pdl_trigger();
   const int G = a.G, tpt = kRows / G;  // tokens per tile
-  const int kvh = blockIdx.y;
 
-  if (warp == kMmaWarp + 1) {
-    // this CTA's sequence and first token: a scan of the sequences' numbers of CTAs
-    int left = blockIdx.x, found = -1, tok0 = 0;
-    for (int s0 = 0; s0 < a.num_seqs && found < 0; s0 += 32) {
-      const int s = s0 + lane;
-      const int ql = s < a.num_seqs ? max(a.cu_q[s + 1] - a.cu_q[s], 0) : 0;
-      const int nb = (ql + 2 * tpt - 1) / (2 * tpt);
-      int inc = nb;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int up = __shfl_up_sync(0xffffffffu, inc, o);
-        if (lane >= o) inc += up;
-      }
-      const uint32_t hit = __ballot_sync(0xffffffffu, left < inc);
-      if (hit != 0) {
-        const int l = __ffs(hit) - 1;
-        const int before = __shfl_sync(0xffffffffu, inc - nb, l), mine = __shfl_sync(0xffffffffu, nb, l);
-        found = s0 + l;
-        tok0 = (mine - 1 - (left - before)) * 2 * tpt;  // the longest prefixes first
-      } else {
-        left -= __shfl_sync(0xffffffffu, inc, 31);
-      }
-    }
+  if (threadIdx.x == 0) a.open_items[blockIdx.x] = make_int4(0, 0, 0, 0);  // rewritten below where one is left
+  if (warp == kMmaWarp) {
+    Cursor c = {};
+    int64_t share;
+    const int count = find_share(a, c, share);
     if (lane == 0) {
-      s_item = Item{found, tok0};
+      s_first = c;
+      s_count = count;
+      s_share = share;
       s_bad = 0;
-      const int ql = found < 0 ? 0 : a.cu_q[found + 1] - a.cu_q[found];
+      s_seen_nan = 0;
+    }
+  }
+  if (warp == kMmaWarp + 1) {
+    if (lane == 0) {
       for (int i = 0; i < kSlots; ++i) {
         mbar_init(&full[i], 1);
-        mbar_init(&empty[i], ql - tok0 > tpt ? 2 : 1);  // the products of every tile have read the slot
+        mbar_init(&empty[i], 2);  // both tiles' warps are done with the slot
       }
       for (int i = 0; i < 2; ++i) {
         mbar_init(&q_full[i], 128);
         for (int h = 0; h < 2; ++h) {  // the steps' parities
           mbar_init(&s_full[i][h], 1);
           mbar_init(&p_ready[i][h], 128);
+          mbar_init(&pv_done[i][h], 1);
         }
-        mbar_init(&pv_done[i], 1);
       }
       fence_barrier_init();
     }
-    if (lane < 8) s_nan[lane] = INT32_MAX;
     __syncwarp();
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem)),
                  "r"(kTmemCols));
@@ -247,74 +414,81 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_fp4_kernel(const __grid_c
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = s_tmem;
-  const Item item = s_item;
-  const int q_start = item.seq < 0 ? 0 : a.cu_q[item.seq];
-  const int q_len = item.seq < 0 ? 0 : a.cu_q[item.seq + 1] - q_start;
-  int kv_len = item.seq < 0 ? 0 : a.kv_lens[item.seq];
-  const int prefix = kv_len - q_len;  // position of the first query
-  if (kv_len > a.cap) {
-    if (threadIdx.x == 0) set_device_status(kStatusBadPage);
-    kv_len = a.cap;
-  }
-  const int n_tok = min(2 * tpt, q_len - item.tok0);  // query tokens of this CTA
-  const int tiles = n_tok > tpt ? 2 : 1;
-  const int last_pos = prefix + item.tok0 + n_tok - 1;  // of the CTA's last query
-  const int n_keys = item.seq < 0 ? 0 : max(0, min(kv_len, last_pos + 1));
-  const int n_kv = (n_keys + kKeys - 1) / kKeys;
-  const int32_t* table = a.tables + (int64_t)max(item.seq, 0) * a.max_blocks;
+  const int count = s_count;
+  Cursor cu = s_first;
 
-  if (item.seq >= 0 && warp < 8) {
+  if (warp < 8) {
     // ------------------------------------------------------------------ softmax
-    const int t = warp >> 2;                                  // tile
-    const int row = (warp & 3) * 32 + lane;                   // TMEM lane
-    const int tt = t * tpt + row / G, h = row % G;            // token of the CTA, head of the group
-    const bool valid = row < tpt * G && tt < n_tok;
-    const int lim = valid ? min(prefix + item.tok0 + tt, kv_len - 1) : -1;  // last visible key
-    if (t < tiles) {
-      const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-      const uint32_t o_addr = lane_base + kColO + t * kD;
-      // Q: 16 lanes a row
-      const int tw = threadIdx.x & 127;
+    const int t = warp >> 2;                        // tile
+    const int row = (warp & 3) * 32 + lane;         // TMEM lane
+    const int tt = t * tpt + row / G, h = row % G;  // token of the item, head of the group
+    const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    const uint32_t o_addr = lane_base + kColO + t * kD;
+    int js = 0;  // steps of this tile so far: the barriers' phases
+    // the item at hand or the next one behind it that has rows in this tile
+    auto find = [&](bool more) {
+      for (; more; more = cu.next_item(a, count)) {
+        if (threadIdx.x == 0 && cu.j0 == 0 && cu.j1 < cu.steps)
+          a.open_items[blockIdx.x] = make_int4((int)((cu.end() - count + s_share - 1) / s_share), cu.s, cu.b, cu.h);
+        if (t * tpt < cu.q.q_len - cu.b * a.tok) return true;
+      }
+      return false;
+    };
+    auto fetch_q = [&] {  // 16 lanes a row
+      const int tw = threadIdx.x & 127, ch = tw & 15, tok0 = cu.b * a.tok;
+      const uint32_t dst = smem_u32(s_q) + (t * 2 + (ch >> 3)) * kQHalf;
+      const __half* src = a.q + (int64_t)(cu.q.q_start + tok0) * a.q_ts + cu.h * G * kD + ch * 8;
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        const int r = (tw >> 4) + 8 * i, ch = tw & 15;
-        const int rt = t * tpt + r / G;
-        uint4 x = make_uint4(0, 0, 0, 0);
-        if (r < tpt * G && rt < n_tok)
-          x = *reinterpret_cast<const uint4*>(a.q + (int64_t)(q_start + item.tok0 + rt) * a.q_ts +
-                                              (kvh * G + r % G) * kD + ch * 8);
-        *reinterpret_cast<uint4*>(s_q + (t * 2 + (ch >> 3)) * kQHalf + r * 128 + (((ch & 7) ^ (r & 7)) << 4)) = x;
+        const int r = (tw >> 4) + 8 * i, rt = (r * a.inv_g) >> 16;  // token of the tile
+        const int qt = t * tpt + rt;
+        const bool in = rt < tpt && qt < min(a.tok, cu.q.q_len - tok0);
+        cp_async16_zfill(dst + r * 128 + (((ch & 7) ^ (r & 7)) << 4), in ? src + qt * a.q_ts + (r - rt * G) * kD : a.q, in);
       }
+    };
+    auto hand_q = [&] {
+      cp_async_wait_all();
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(&q_full[t]);
-      int low = lim;  // smallest limit of the warp: tiles below it need no mask
+    };
+    bool more = find(count > 0);
+    if (more) {
+      fetch_q();
+      hand_q();
+    }
+    while (more) {
+      const int j0 = cu.j0, j1 = cu.j1;
+      const bool whole = j0 == 0 && j1 == cu.steps;
+      const int tok0 = cu.b * a.tok, n_tok = min(a.tok, cu.q.q_len - tok0);
+      const bool valid = row < tpt * G && tt < n_tok;
+      const int lim = valid ? min(cu.q.prefix + tok0 + tt, cu.q.kv_len - 1) : -1;  // last visible key
+      const int seq = cu.s, kvh = cu.h, seen_end = min(j1 * kKeys, cu.keys);
+      const int64_t out_row = ((int64_t)(cu.q.q_start + tok0 + tt) * a.Hkv + kvh) * G + h;
+      int low = lim;  // smallest limit of the warp: steps below it need no mask
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) low = min(low, __shfl_xor_sync(0xffffffffu, low, o));
       float m = -INFINITY, l = 0.f;  // reference (log2 units, less kPScaleLog2) and sum
       bool ok = true;
-      for (int j = 0; j < n_kv; ++j) {
-        if (!mbar_wait(&s_full[t][j & 1], (j >> 1) & 1)) {
-          ok = false;
-          break;
-        }
+      for (int j = j0; j < j1; ++j, ++js) {
+        ok = warp_wait(&s_full[t][js & 1], (js >> 1) & 1);
+        if (!ok) break;
         tc_fence_after();
         const int kbase = j * kKeys;
-        const uint32_t s_addr = lane_base + t * 128 + (j & 1) * kKeys;
-        const bool masked = kbase + kKeys - 1 > low || *reinterpret_cast<volatile int*>(&s_bad) != 0;
+        const uint32_t s_addr = lane_base + t * 128 + (js & 1) * kKeys;
+        const bool bad = *reinterpret_cast<volatile int*>(&s_bad) != 0;
         // ---- the row's 64 scores, and their maximum ---------------------------------------------
         float v[2][32];
 #pragma unroll
         for (int c = 0; c < 2; ++c) tmem_ld32(s_addr + 32 * c, v[c]);
         tmem_ld_wait();
-        if (masked) {
-          const bool bad = *reinterpret_cast<volatile int*>(&s_bad) != 0;
+        if (kbase + kKeys - 1 > low || bad) {
 #pragma unroll
           for (int c = 0; c < 2; ++c) {
             const int k0 = kbase + 32 * c, n = lim - k0 + 1;  // keys of these 32 that the row sees
             uint32_t seen = n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u);
             if (bad) {  // rare: leave out the keys of bad pages
               const int pg = k0 / a.block_size;
-              const int64_t blk = pg < a.max_blocks ? table[pg] : -1;
+              const int64_t blk = pg < a.max_blocks ? a.tables[(int64_t)seq * a.max_blocks + pg] : -1;
               if (blk < 0 || blk >= a.num_blocks) seen = 0;
             }
             hide(v[c], seen);
@@ -328,11 +502,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_fp4_kernel(const __grid_c
           const float al = m == -INFINITY ? 1.f : ex2(m - mn);
           m = mn;
           l *= al;
-          if (j > 0) {
-            if (!mbar_wait(&pv_done[t], (j - 1) & 1)) {
-              ok = false;
-              break;
-            }
+          if (j > j0) {
+            // S of this step was issued behind the product of step js - 2, so the phase of this barrier before
+            // the awaited one is over
+            ok = warp_wait(&pv_done[t][(js - 1) & 1], ((js - 1) >> 1) & 1);
+            if (!ok) break;
             tc_fence_after();
 #pragma unroll
             for (int c = 0; c < 8; ++c) {
@@ -366,50 +540,65 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_fp4_kernel(const __grid_c
         }
         tmem_st_wait();
         tc_fence_before();
-        mbar_arrive(&p_ready[t][j & 1]);
-        {
-          float x0, x1;
-          unpack2(add2(sum[0], sum[1]), x0, x1);
-          l += x0 + x1;
-        }
+        mbar_arrive(&p_ready[t][js & 1]);
+        float x0, x1;
+        unpack2(add2(sum[0], sum[1]), x0, x1);
+        l += x0 + x1;
       }
-      // ---- O / l ----------------------------------------------------------------------------------
-      if (ok && n_kv > 0) {
-        ok = mbar_wait(&pv_done[t], (n_kv - 1) & 1);
-        tc_fence_after();
-      }
-      role_sync();  // every V tile has been decoded: s_nan is complete
-      const float inv = l == 0.f ? 0.f : 1.f / l;
-      __half* dst = a.out + ((int64_t)(q_start + item.tok0 + tt) * a.Hkv * G + kvh * G + h) * kD;
+      if (!ok) break;
+      // Q is no longer read: fetch the next item's under the last product, so that its first scores are made
+      // under this item's end
+      more = find(cu.next_item(a, count));
+      if (more) fetch_q();
+      // The last product. S of its step was issued before the product of step js - 2, which may still run,
+      // hence a barrier per parity of steps: one for both could not tell the two by its phase.
+      ok = warp_wait(&pv_done[t][(js - 1) & 1], ((js - 1) >> 1) & 1);
+      if (more) hand_q();
+      if (!ok) break;
+      tc_fence_after();
+      // ---- the item's steps of this CTA are done: O / l, or a partial ------------------------------
+      uint32_t nan = 0;  // 16-element groups in which this row sees a NaN of V
+      if (__any_sync(0xffffffffu, *reinterpret_cast<volatile int*>(&s_seen_nan) != 0))
+        nan = nan_groups(a, seq, kvh, j0 * kKeys, seen_end, lim);
+      const float qnan = __int_as_float(0x7fffffff);
+      if (whole) {
+        const float inv = l == 0.f ? 0.f : 1.f / l;
+        __half* dst = a.out + out_row * kD;
 #pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        float v[32];
-        if (n_kv > 0) {
-          tmem_ld32(o_addr + 32 * c, v);
+        for (int c = 0; c < 4; ++c) {
+          float o[32];
+          tmem_ld32(o_addr + 32 * c, o);
           tmem_ld_wait();
-        } else {
+          if (valid) {
 #pragma unroll
-          for (int i = 0; i < 32; ++i) v[i] = 0.f;
-        }
-        if (ok && valid) {
-#pragma unroll
-          for (int g2 = 0; g2 < 2; ++g2) {
-            const float f = s_nan[2 * c + g2] <= lim ? __int_as_float(0x7fffffff) : inv;
-#pragma unroll
-            for (int i = 0; i < 16; i += 8) {
-              const float* x = v + 16 * g2 + i;
-              *reinterpret_cast<uint4*>(dst + 32 * c + 16 * g2 + i) =
-                  make_uint4(pack_h2(x[0] * f, x[1] * f), pack_h2(x[2] * f, x[3] * f), pack_h2(x[4] * f, x[5] * f),
-                             pack_h2(x[6] * f, x[7] * f));
+            for (int i = 0; i < 32; i += 8) {
+              const float f = (nan >> (2 * c + (i >> 4))) & 1u ? qnan : inv;
+              *reinterpret_cast<uint4*>(dst + 32 * c + i) =
+                  make_uint4(pack_h2(o[i] * f, o[i + 1] * f), pack_h2(o[i + 2] * f, o[i + 3] * f),
+                             pack_h2(o[i + 4] * f, o[i + 5] * f), pack_h2(o[i + 6] * f, o[i + 7] * f));
             }
           }
         }
+      } else {  // slot 0: the item began in an earlier CTA; slot 1: it begins here and goes on
+        float* part = a.ws + ((int64_t)blockIdx.x * 2 + (j0 > 0 ? 0 : 1)) * kPartFloats;
+        const int pr = t * kRows + row;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          float o[32];
+          tmem_ld32(o_addr + 32 * c, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; i += 4) {
+            const float f = (nan >> (2 * c + (i >> 4))) & 1u ? qnan : 1.f;
+            *reinterpret_cast<float4*>(part + ((8 * c + (i >> 2)) * kPartRows + pr) * 4) =
+                make_float4(o[i] * f, o[i + 1] * f, o[i + 2] * f, o[i + 3] * f);
+          }
+        }
+        *reinterpret_cast<float2*>(part + kPartRows * kD + pr * 2) = make_float2(m, l);
       }
-    } else {
-      role_sync();
+      tc_fence_before();  // O is read before the next item's first product, which waits for p_ready
     }
-  } else if (item.seq >= 0) {
-    if (warp < kMmaWarp) {
+  } else if (warp < kMmaWarp) {
     // ------------------------------------------------------------------ decode of K and V
     // a lane's part of a slot: rows lr + 8 i, elements 64 half + 32 c2 .. + 32 of each
     const int lr = (lane >> 1) & 7, c2 = lane & 1, half = lane >> 4;
@@ -422,15 +611,19 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_fp4_kernel(const __grid_c
     // before that, which (releases keep the order, but for neighbours) came after the release
     // of the use before the last of this slot.
     static_assert(kSlots > kDecodeWarps, "parity of the slots' uses");
-    for (int n = warp - 8; n < 2 * n_kv; n += kDecodeWarps) {  // K (n even) or V (odd) of step n / 2
-      const int k0 = (n >> 1) * kKeys;
+    bool more = count > 0;
+    for (int n = warp - 8;; n += kDecodeWarps) {  // K (n even) or V (odd) of the CTA's step n / 2
+      while (more && (n >> 1) >= cu.first + cu.j1 - cu.j0) more = cu.next_item(a, count);
+      if (!more) break;
+      const int k0 = ((n >> 1) - cu.first + cu.j0) * kKeys;
       const int page = a.bs_log2 >= 0 ? k0 >> a.bs_log2 : k0 / a.block_size;
-      const int64_t blk = page < a.max_blocks ? __ldg(table + page) : -1;
+      const int64_t blk =
+          k0 < cu.keys && page < a.max_blocks ? __ldg(a.tables + (int64_t)cu.s * a.max_blocks + page) : -1;
       const bool live = blk >= 0 && blk < a.num_blocks;
       uint4 codes[kKeys / 8];
       uint32_t sc[kKeys / 8];  // two scale bytes; 0: zeros, whatever the codes
       if (live) {
-        const int64_t r0 = (blk * a.Hkv + kvh) * a.block_size + (k0 - page * a.block_size) + lr;
+        const int64_t r0 = (blk * a.Hkv + cu.h) * a.block_size + (k0 - page * a.block_size) + lr;
         const uint8_t* cp = ((n & 1) ? a.vc : a.kc) + r0 * kFp4RowBytes + half * 32 + c2 * 16;
         const uint8_t* sp = ((n & 1) ? a.vs : a.ks) + r0 * kFp4ScaleBytes + half * 4 + c2 * 2;
 #pragma unroll
@@ -438,14 +631,16 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_fp4_kernel(const __grid_c
           codes[i] = __ldg(reinterpret_cast<const uint4*>(cp + i * 8 * kFp4RowBytes));
           sc[i] = __ldg(reinterpret_cast<const uint16_t*>(sp + i * 8 * kFp4ScaleBytes));
         }
-        if (k0 + kKeys > n_keys) {
+        if (k0 + kKeys > cu.keys) {
 #pragma unroll
           for (int i = 0; i < kKeys / 8; ++i)
-            if (k0 + lr + 8 * i >= n_keys) sc[i] = 0;
+            if (k0 + lr + 8 * i >= cu.keys) sc[i] = 0;
         }
       } else {
-        set_device_status(kStatusBadPage);
-        s_bad = 1;
+        if (k0 < cu.keys) {
+          set_device_status(kStatusBadPage);
+          s_bad = 1;
+        }
 #pragma unroll
         for (int i = 0; i < kKeys / 8; ++i) {
           codes[i] = make_uint4(0, 0, 0, 0);
@@ -453,22 +648,16 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_fp4_kernel(const __grid_c
         }
       }
       const int slot = n % kSlots;
-      if (!mbar_wait(&empty[slot], ((n / kSlots) & 1) ^ 1)) break;
+      if (!warp_wait(&empty[slot], ((n / kSlots) & 1) ^ 1)) break;
       unsigned char* dst = s_kv + slot * kSlotBytes;
 #pragma unroll
       for (int i = 0; i < kKeys / 8; ++i) {
         uint32_t s = sc[i];
         if ((n & 1) && ((s & 0xF8u) == 0xF8u || (s & 0xF800u) == 0xF800u)) {
           // V: no NaN (or infinity) reaches the product
-          const int key = k0 + lr + 8 * i;
-          if ((s & 0xF8u) == 0xF8u) {
-            atomicMin(&s_nan[4 * half + 2 * c2], key);
-            s &= 0xFF00u;
-          }
-          if ((s & 0xF800u) == 0xF800u) {
-            atomicMin(&s_nan[4 * half + 2 * c2 + 1], key);
-            s &= 0xFFu;
-          }
+          s_seen_nan = 1;
+          if ((s & 0xF8u) == 0xF8u) s &= 0xFF00u;
+          if ((s & 0xF800u) == 0xF800u) s &= 0xFFu;
         }
         const uint32_t f[2] = {fp4_scale_h2(s & 0xFFu), fp4_scale_h2(s >> 8)};
         const uint32_t cw[4] = {codes[i].x, codes[i].y, codes[i].z, codes[i].w};
@@ -484,74 +673,86 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_fp4_kernel(const __grid_c
       __syncwarp();
       if (lane == 0) mbar_arrive(&full[slot]);
     }
-    __syncwarp();
-    role_sync();
-    } else {
+  } else {
     // ------------------------------------------------------------------ MMA issue
     // The whole warp walks the loop, so that descriptors and addresses stay in uniform registers, and
     // one lane's products and commits count: issued by one thread in a divergent branch, a product took
     // some 70 cycles to issue, more than to run.
     const int t = warp - kMmaWarp;  // tile
-    if (t < tiles && n_kv > 0) {
-      const uint32_t lead = elect_one();
-      const uint32_t kv0 = smem_u32(s_kv);
-      const uint64_t dq = desc_base(smem_u32(s_q) + t * 2 * kQHalf, 16);
-      // slot number n is stage n % kSlots in its use n / kSlots
-      auto wait_full = [&](int stage, int use) { return mbar_wait(&full[stage], use & 1); };
-      auto scores = [&](int stage, int j) {  // S = Q K_j^T
-        const uint64_t dk = desc_base(kv0 + stage * kSlotBytes, 16);
-        const uint32_t d = tmem + t * 128 + (j & 1) * kKeys;
+    const uint32_t lead = elect_one();
+    const uint32_t kv0 = smem_u32(s_kv);
+    const uint64_t dq = desc_base(smem_u32(s_q) + t * 2 * kQHalf, 16);
+    auto scores = [&](int stage, int js) {  // S = Q K^T
+      const uint64_t dk = desc_base(kv0 + stage * kSlotBytes, 16);
+      const uint32_t d = tmem + t * 128 + (js & 1) * kKeys;
 #pragma unroll
-        for (int k = 0; k < 8; ++k)  // 16 elements each
-          mma_ss(d, dq + (uint64_t)(((k >> 2) * kQHalf + (k & 3) * 32) >> 4),
-                 dk + (uint64_t)(((k >> 2) * kHalf + (k & 3) * 32) >> 4), kIdescQK, k > 0, lead);
-        mma_commit(&s_full[t][j & 1], lead);
-      };
-      // nobody waits for the last slots: no arrival may outlive the CTA
-      const int last_release = 2 * n_kv - kSlots;
-      bool ok = mbar_wait(&q_full[t], 0) && wait_full(0, 0);
-      if (ok) {
-        tc_fence_after();
-        scores(0, 0);
-        if (0 < last_release) mma_commit(&empty[0], lead);
+      for (int k = 0; k < 8; ++k)  // 16 elements each
+        mma_ss(d, dq + (uint64_t)(((k >> 2) * kQHalf + (k & 3) * 32) >> 4),
+               dk + (uint64_t)(((k >> 2) * kHalf + (k & 3) * 32) >> 4), kIdescQK, k > 0, lead);
+      mma_commit(&s_full[t][js & 1], lead);
+    };
+    // the next K and the next V: slot of the ring, parity of its use
+    struct Place {
+      int stage, par;
+    } k = {0, 0}, v = {1, 0};
+    static_assert(kSlots % 2 == 0 && kSlots > 2, "K and V keep their parity of stages");
+    auto release = [&](Place& p) {  // by a commit even without products: the warp's releases keep their order
+      mma_commit(&empty[p.stage], lead);
+      p.stage += 2;
+      if (p.stage >= kSlots) {
+        p.stage -= kSlots;
+        p.par ^= 1;
       }
-      int kst = 2 % kSlots, kuse = 0, vst = 1, vuse = 0;  // stages and uses of K_{j+1} and V_j
-      static_assert(kSlots % 2 == 0 && kSlots > 2, "K and V keep their parity of stages");
-      for (int j = 0; ok && j < n_kv; ++j) {
-        if (j + 1 < n_kv) {
-          // S of the next step: its buffer held the weights of step j - 1, whose product was issued before
-          ok = wait_full(kst, kuse);
+    };
+    int js = 0, items = 0;
+    bool ok = true;
+    for (bool more = count > 0; more; more = cu.next_item(a, count)) {
+      const int j0 = cu.j0, j1 = cu.j1;
+      if (t * tpt >= min(a.tok, cu.q.q_len - cu.b * a.tok)) {  // no rows in this tile: pass the slots on
+        for (int j = j0; ok && j < j1; ++j) {
+          ok = warp_wait(&full[k.stage], k.par);
+          if (ok) release(k);
+          ok = ok && warp_wait(&full[v.stage], v.par);
+          if (ok) release(v);
+        }
+        if (!ok) break;
+        continue;
+      }
+      ok = warp_wait(&q_full[t], items & 1) && warp_wait(&full[k.stage], k.par);
+      if (!ok) break;
+      ++items;
+      tc_fence_after();
+      scores(k.stage, js);
+      release(k);
+      for (int j = j0; j < j1; ++j, ++js) {
+        if (j + 1 < j1) {
+          // S of the next step: its buffer held the weights of step js - 1, whose product was issued before
+          ok = warp_wait(&full[k.stage], k.par);
           if (!ok) break;
           tc_fence_after();
-          scores(kst, j + 1);
-          if (2 * j + 2 < last_release) mma_commit(&empty[kst], lead);
-          kst += 2;
-          if (kst >= kSlots) {
-            kst -= kSlots;
-            ++kuse;
-          }
+          scores(k.stage, js + 1);
+          release(k);
         }
-        ok = wait_full(vst, vuse) && mbar_wait(&p_ready[t][j & 1], (j >> 1) & 1);
+        ok = warp_wait(&full[v.stage], v.par) && warp_wait(&p_ready[t][js & 1], (js >> 1) & 1);
         if (!ok) break;
         tc_fence_after();
-        const uint64_t dv = desc_base(kv0 + vst * kSlotBytes, kHalf);
-        const uint32_t p = tmem + t * 128 + (j & 1) * kKeys;
+        const uint64_t dv = desc_base(kv0 + v.stage * kSlotBytes, kHalf);
+        const uint32_t p = tmem + t * 128 + (js & 1) * kKeys;
 #pragma unroll
-        for (int k = 0; k < kKeys / 16; ++k)  // 16 keys each
-          mma_ts(tmem + kColO + t * kD, p + 8 * k, dv + (uint64_t)((k * 2048) >> 4), kIdescPV, j > 0 || k > 0, lead);
-        mma_commit(&pv_done[t], lead);
-        if (2 * j + 1 < last_release) mma_commit(&empty[vst], lead);
-        vst += 2;
-        if (vst >= kSlots) {
-          vst -= kSlots;
-          ++vuse;
-        }
+        for (int i = 0; i < kKeys / 16; ++i)  // 16 keys each
+          mma_ts(tmem + kColO + t * kD, p + 8 * i, dv + (uint64_t)((i * 2048) >> 4), kIdescPV, j > j0 || i > 0, lead);
+        mma_commit(&pv_done[t][js & 1], lead);
+        release(v);
       }
+      if (!ok) break;
     }
-    __syncwarp();
-    role_sync();
+    // no arrival may outlive the CTA: wait for the release of each slot's last use (the places point behind it)
+    for (int i = 0; ok && i < kSlots; ++i) {
+      const Place& p = (i & 1) ? v : k;
+      ok = warp_wait(&empty[i], i < p.stage ? p.par : p.par ^ 1);
     }
   }
+  __syncwarp();
   tc_fence_before();
   __syncthreads();
   if (warp == kMmaWarp + 1) {
@@ -560,25 +761,73 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_fp4_kernel(const __grid_c
   }
 }
 
-}  // namespace
-
-cudaError_t prefill_fp4_take_status(int* host, cudaStream_t stream) {
-  static const int zero = 0;
-  cudaError_t e = cudaMemcpyFromSymbolAsync(host, g_device_status, sizeof(int), 0, cudaMemcpyDeviceToHost, stream);
-  if (e == cudaSuccess)
-    e = cudaMemcpyToSymbolAsync(g_device_status, &zero, sizeof(int), 0, cudaMemcpyHostToDevice, stream);
-  return e;
+// Items that cross CTAs: block (i, y) joins 32 rows of the one that CTA i leaves open, if any, from its
+// partial there (slot 1) and those of the CTAs behind it (slot 0). A lane has a row, a warp 16 elements.
+constexpr int kMergeThreads = 256;
+__global__ void __launch_bounds__(kMergeThreads) merge_prefill_fp4_kernel(const __grid_constant__ PrefillArgs a) {
+  pdl_wait();
+  pdl_trigger();
+  const int4 item = a.open_items[blockIdx.x];
+  const int n = min(item.x, (int)(gridDim.x - blockIdx.x));  // partials behind the first
+  if (n <= 0) return;
+  const int row = blockIdx.y * 32 + (threadIdx.x & 31), e0 = (threadIdx.x >> 5) * 16;
+  const int tpt = kRows / a.G, r = row % kRows, tt = row / kRows * tpt + r / a.G;
+  const Seq q = seq_of(a, item.y);
+  const int tok = item.z * a.tok + tt;
+  if (r >= tpt * a.G || tok >= q.q_len) return;
+  float M = -INFINITY, L = 0.f, o[16];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) o[i] = 0.f;
+#pragma unroll 2
+  for (int j = 0; j <= n; ++j) {
+    const float* part = a.ws + ((int64_t)(blockIdx.x + j) * 2 + (j == 0 ? 1 : 0)) * kPartFloats;
+    const float2 ml = *reinterpret_cast<const float2*>(part + kPartRows * kD + row * 2);
+    float4 u[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+      u[i] = *reinterpret_cast<const float4*>(part + ((e0 / 4 + i) * kPartRows + row) * 4);
+    const float mn = fmaxf(M, ml.x);
+    const float w0 = M == -INFINITY ? 1.f : ex2(M - mn), w1 = ml.x == -INFINITY ? 1.f : ex2(ml.x - mn);
+    M = mn;
+    L = L * w0 + ml.y * w1;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      o[4 * i] = o[4 * i] * w0 + u[i].x * w1;
+      o[4 * i + 1] = o[4 * i + 1] * w0 + u[i].y * w1;
+      o[4 * i + 2] = o[4 * i + 2] * w0 + u[i].z * w1;
+      o[4 * i + 3] = o[4 * i + 3] * w0 + u[i].w * w1;
+    }
+  }
+  const float f = L == 0.f ? 0.f : 1.f / L;
+  __half* dst = a.out + ((int64_t)(q.q_start + tok) * a.Hkv * a.G + item.w * a.G + r % a.G) * kD + e0;
+#pragma unroll
+  for (int i = 0; i < 16; i += 8)
+    *reinterpret_cast<uint4*>(dst + i) =
+        make_uint4(pack_h2(o[i] * f, o[i + 1] * f), pack_h2(o[i + 2] * f, o[i + 3] * f),
+                   pack_h2(o[i + 4] * f, o[i + 5] * f), pack_h2(o[i + 6] * f, o[i + 7] * f));
 }
 
-cudaError_t prefill_fp4_set_wait_limit(unsigned long long ns) {
-  return cudaMemcpyToSymbol(g_wait_limit_ns, &ns, sizeof(ns));
+// One CTA per SM; fewer when even full tables would not give every CTA kMinShare units.
+int prefill_fp4_ctas(int num_seqs, int total_q, int Hkv, int G, int max_blocks, int block_size, int num_sms) {
+  const int64_t items = ((int64_t)total_q / (2 * (kRows / G)) + num_seqs) * Hkv;
+  const int64_t units = items * ((int64_t)max_blocks * (block_size / kKeys) + kItemUnits);
+  const int64_t need = (units + kMinShare - 1) / kMinShare;
+  return (int)(need < num_sms ? (need > 0 ? need : 1) : num_sms);
+}
+
+}  // namespace
+
+size_t prefill_fp4_workspace_bytes(int num_seqs, int total_q, int Hq, int Hkv, int max_blocks, int block_size,
+                                   int num_sms) {
+  const int ctas = prefill_fp4_ctas(num_seqs, total_q, Hkv, Hq / Hkv, max_blocks, block_size, num_sms);
+  return (size_t)ctas * (sizeof(int4) + 2 * kPartFloats * sizeof(float));
 }
 
 cudaError_t launch_prefill_fp4(const void* q, int64_t q_ts, const void* k_cache, const void* v_cache,
                                const void* k_scale, const void* v_scale, int64_t num_blocks,
                                const int32_t* block_tables, const int32_t* cu_q, const int32_t* kv_lens, void* out,
                                int num_seqs, int total_q, int Hq, int Hkv, int block_size, int max_blocks,
-                               float softmax_scale, cudaStream_t stream) {
+                               float softmax_scale, void* workspace, int num_sms, cudaStream_t stream) {
   PrefillArgs a = {};
   a.q = (const __half*)q;
   a.q_ts = q_ts;
@@ -595,22 +844,29 @@ cudaError_t launch_prefill_fp4(const void* q, int64_t q_ts, const void* k_cache,
   a.total_q = total_q;
   a.Hkv = Hkv;
   a.G = Hq / Hkv;
+  a.inv_g = (65536 + a.G - 1) / a.G;
+  a.tok = 2 * (kRows / a.G);
   a.block_size = block_size;
   a.bs_log2 = (block_size & (block_size - 1)) == 0 ? __builtin_ctz((unsigned)block_size) : -1;
   a.max_blocks = max_blocks;
   const int64_t cap = (int64_t)max_blocks * block_size;
   a.cap = (int)(cap < (1 << 30) ? cap : (1 << 30));
   a.scale_log2 = softmax_scale * kLog2e;
-  const int tpc = 2 * (kRows / a.G);
-  // CTAs over all sequences: sum ceil(len / tpc) <= total / tpc + sequences
-  const int64_t blocks = (int64_t)total_q / tpc + num_seqs;
+  // sums of units fit 32 bits in the kernel
+  if (((int64_t)total_q / a.tok + num_seqs) * (a.cap / kKeys + 1 + kItemUnits) >= ((int64_t)1 << 31) / Hkv)
+    return cudaErrorInvalidValue;
+  const int ctas = prefill_fp4_ctas(num_seqs, total_q, Hkv, a.G, max_blocks, block_size, num_sms);
+  a.open_items = (int4*)workspace;
+  a.ws = (float*)((int4*)workspace + ctas);
   static std::once_flag once;
   static cudaError_t attr = cudaSuccess;
   std::call_once(once, [] {
     attr = cudaFuncSetAttribute(prefill_fp4_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
   });
   if (attr != cudaSuccess) return attr;
-  return launch_kernel(prefill_fp4_kernel, dim3((unsigned)blocks, (unsigned)Hkv), dim3(kThreads), kSmemBytes, stream, a);
+  const cudaError_t e = launch_kernel(prefill_fp4_kernel, dim3(ctas), dim3(kThreads), kSmemBytes, stream, a);
+  if (e != cudaSuccess || ctas == 1) return e;
+  return launch_kernel(merge_prefill_fp4_kernel, dim3(ctas - 1, kPartRows / 32), dim3(kMergeThreads), 0, stream, a);
 }
 
 }  // namespace ms

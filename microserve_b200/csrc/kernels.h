@@ -54,14 +54,13 @@ cudaError_t launch_decode_fp4(const void* q, int64_t q_ts, const void* k_cache, 
                               const void* k_scale, const void* v_scale, int64_t num_blocks, const int32_t* seqlens,
                               const int32_t* block_tables, void* out, int B, int Hq, int Hkv, int block_size,
                               int max_blocks, float softmax_scale, void* workspace, int num_sms, cudaStream_t stream);
-// The status word and wait limit of fp4_prefill_attn.cu (common.cuh: MS_WHOLE_PROGRAM).
-cudaError_t prefill_fp4_take_status(int* host, cudaStream_t stream);
-cudaError_t prefill_fp4_set_wait_limit(unsigned long long ns);
+size_t prefill_fp4_workspace_bytes(int num_seqs, int total_q, int Hq, int Hkv, int max_blocks, int block_size,
+                                   int num_sms);
 cudaError_t launch_prefill_fp4(const void* q, int64_t q_ts, const void* k_cache, const void* v_cache,
                                const void* k_scale, const void* v_scale, int64_t num_blocks,
                                const int32_t* block_tables, const int32_t* cu_q, const int32_t* kv_lens, void* out,
                                int num_seqs, int total_q, int Hq, int Hkv, int block_size, int max_blocks,
-                               float softmax_scale, cudaStream_t stream);
+                               float softmax_scale, void* workspace, int num_sms, cudaStream_t stream);
 
 cudaError_t launch_copy_pages(void* cache, int64_t cache_plane_stride, int row_bytes, void* scale,
                               int64_t scale_plane_stride, int scale_row_bytes, int planes, int outer, int block_size,

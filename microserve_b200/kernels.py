@@ -455,10 +455,14 @@ def paged_prefill_fp4(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     _int32("paged_prefill_fp4", "block_tables", block_tables, num_seqs, -1)
     query, q_stride, o = _fp4_query("paged_prefill_fp4", query, out)
     _on_current_device("paged_prefill_fp4", query, k_cache, v_cache, k_scale, v_scale, block_tables, cu_q, kv_lens, o)
-    check(_lib.load().ms_paged_prefill_fp4(query.data_ptr(), q_stride, k_cache.data_ptr(), v_cache.data_ptr(),
-                                           k_scale.data_ptr(), v_scale.data_ptr(), NB, block_tables.data_ptr(),
-                                           cu_q.data_ptr(), kv_lens.data_ptr(), o.data_ptr(), num_seqs, T, Hq, Hkv,
-                                           D, BS, block_tables.shape[1], float(softmax_scale), stream_ptr()),
+    lib = _lib.load()
+    max_blocks = block_tables.shape[1]
+    ws = torch.empty(lib.ms_paged_prefill_fp4_workspace_size(num_seqs, T, Hq, Hkv, max_blocks, BS), dtype=torch.uint8,
+                     device=query.device)  # its own for every call, as in paged_decode_fp4
+    check(lib.ms_paged_prefill_fp4(query.data_ptr(), q_stride, k_cache.data_ptr(), v_cache.data_ptr(),
+                                   k_scale.data_ptr(), v_scale.data_ptr(), NB, block_tables.data_ptr(),
+                                   cu_q.data_ptr(), kv_lens.data_ptr(), o.data_ptr(), num_seqs, T, Hq, Hkv, D, BS,
+                                   max_blocks, float(softmax_scale), ws.data_ptr(), ws.numel(), stream_ptr()),
           "ms_paged_prefill_fp4")
     return o
 

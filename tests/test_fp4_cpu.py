@@ -26,9 +26,9 @@ def _decode(q=P, qs=2048, cache=P, blocks=4, lens=P, tables=P, B=2, Hq=16, Hkv=8
 
 
 def _prefill(q=P, qs=2048, cache=P, blocks=4, tables=P, cu=P, n=2, T=9, Hq=16, Hkv=8, dim=128, bs=256, mb=4,
-             scale=0.1):
+             scale=0.1, ws=P, wb=1 << 40):
     return _lib.load().ms_paged_prefill_fp4(q, qs, cache, P, P, P, blocks, tables, cu, P, P, n, T, Hq, Hkv, dim, bs,
-                                            mb, scale, None)
+                                            mb, scale, ws, wb, None)
 
 
 def _copy(cache=P, cs=1 << 30, row=1024, scale=P, ss=1 << 30, srow=32, planes=2, outer=1, bs=256, pages=8, src=P,
@@ -52,6 +52,8 @@ INVALID, UNSUPPORTED = _lib.MS_ERR_INVALID, _lib.MS_ERR_UNSUPPORTED
     (_decode, dict(ws=None), _lib.MS_ERR_WORKSPACE), (_decode, dict(wb=100), _lib.MS_ERR_WORKSPACE),
     (_decode, dict(ws=P + 8), INVALID), (_decode, dict(scale=0.0), INVALID), (_decode, dict(scale=-1.0), INVALID),
     (_decode, dict(scale=float("nan")), INVALID), (_prefill, dict(scale=float("inf")), INVALID),
+    (_prefill, dict(ws=None), _lib.MS_ERR_WORKSPACE), (_prefill, dict(wb=64), _lib.MS_ERR_WORKSPACE),
+    (_prefill, dict(ws=P + 8), INVALID),
     (_prefill, dict(n=0), 0), (_prefill, dict(T=0), 0), (_prefill, dict(T=1 << 31), INVALID),
     (_prefill, dict(Hq=9), UNSUPPORTED), (_prefill, dict(cu=None), INVALID), (_prefill, dict(q=None), INVALID),
     (_prefill, dict(bs=100), UNSUPPORTED), (_prefill, dict(Hkv=0), INVALID),
