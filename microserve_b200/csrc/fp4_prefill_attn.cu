@@ -8,22 +8,25 @@
 // keys that both tiles read. The steps of all items (sequence, block of tokens, kv head) form
 // one list that is dealt evenly to one CTA per SM, whatever the lengths are; an item that
 // crosses CTAs leaves fp32 partials (O, reference, sum) in the workspace, joined by a second kernel.
+// 2048 queries behind 30720 tokens (32 / 8 heads) take 997 us, 1068 TFLOP/s of visible pairs.
 // The roles below walk a CTA's items on their own, so decoding runs ahead into the next one.
 //   warps 0-3, 4-7   softmax of tile 0 / 1: a thread owns a row. It reads its 64 scores of a
 //                    step from TMEM, writes the weights over them as f16, and keeps the row's
-//                    maximum and sum (fp32).
+//                    maximum and sum (fp32). Its registers are full, so an item's numbers come
+//                    from shared memory where they are needed (kept in registers: 1141 us).
 //   warps 8-13       decode K and V codes to f16 in shared memory (128-byte swizzle), a
 //                    ring of kSlots 16 KB slots in the order K0 V0 K1 V1 ..., a warp a slot:
 //                    the fence between its stores and the tensor core's reads and the
-//                    barriers cost as much as 16 keys' work (16 keys a turn: 1.34 ms).
-//   warps 14, 15     each issues one tile's S = Q K^T (both in shared memory, K-major) and
-//                    O += P V (P from TMEM, V as it lies in the cache: MN-major). One warp for
-//                    both tiles spends 1.6 thousand cycles a step on waits and issue, the
-//                    tensor core needs 1.24. Warp 15 allocates TMEM.
+//                    barriers cost as much as 16 keys' work.
+//   warps 14, 15     each walks the items of one tile, fetches Q by TMA, and issues S = Q K^T (both
+//                    in shared memory, K-major) and O += P V (P from TMEM, V as it lies in the cache:
+//                    MN-major). One warp for both tiles spends 1.6 thousand cycles a step on waits and
+//                    issue, the tensor core needs 1.24. The next item's Q and first scores are made
+//                    under the last product and the output of the one at hand. Warp 15 allocates TMEM.
 // The scores are double-buffered (TMEM: two tiles x two S of 64 columns, two O of 128), so S of
 // the next step is there when a softmax ends and the chain S -> softmax -> P V of a tile never
 // stalls its softmax warps: with one S a tile (128 keys a step, or 64 and Q in TMEM) the
-// chain's latencies showed, 1.11 and 1.25 ms for 2048 queries on 30720 tokens.
+// chain's latencies show, 4 and 16 % more time.
 // Softmax in the exp2 domain against a lazy reference: weights are 2^(s - m) for a reference
 // m that moves, with a rescale of O in TMEM, only when a row's maximum exceeds it by 8 or
 // more. Weights are rounded to f16 for the second product (2^-11 relative; the first
@@ -37,6 +40,7 @@
 
 #include "fp4_kv.cuh"
 #include "kernels.h"
+#include "tensor_map.h"
 
 namespace ms {
 namespace {
@@ -162,10 +166,32 @@ __device__ __forceinline__ void tmem_ld16(uint32_t addr, float (&v)[16]) {
       : "r"(addr));
 }
 
-__device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool in) {  // not in: zeros
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
+__device__ __forceinline__ void tma_load_3d(const CUtensorMap* map, uint32_t dst, uint64_t* bar, int c0, int c1,
+                                            int c2) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::
+          "r"(dst),
+      "l"(map), "r"(c0), "r"(c1), "r"(c2), "r"(smem_u32(bar))
+      : "memory");
 }
-__device__ __forceinline__ void cp_async_wait_all() { asm volatile("cp.async.wait_all;" ::: "memory"); }
+// Lanes 4 i .. 4 i + 3 hold a row each, as four pieces of 16 bytes: afterwards lane 4 i + k has piece k of all four.
+__device__ __forceinline__ void transpose4(uint32_t (&p)[16]) {
+#pragma unroll
+  for (int b = 1; b <= 2; b <<= 1) {
+    const bool up = threadIdx.x & b;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (j & b) continue;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        uint32_t &lo = p[4 * j + w], &hi = p[4 * (j ^ b) + w];
+        const uint32_t got = __shfl_xor_sync(0xffffffffu, up ? lo : hi, b);
+        lo = up ? got : lo;
+        hi = up ? hi : got;
+      }
+    }
+  }
+}
 
 // mbar_wait by a whole warp, with one answer (lanes may run out of time at different moments).
 __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t phase) {
@@ -173,8 +199,6 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t phase) {
 }
 
 struct PrefillArgs {
-  const __half* q;  // [T, Hq, D], token stride q_ts elements
-  int64_t q_ts;
   const uint8_t *kc, *vc, *ks, *vs;
   int64_t num_blocks;
   const int32_t* tables;  // [S, max_blocks]
@@ -189,10 +213,13 @@ struct PrefillArgs {
   float scale_log2;
 };
 
-// The list is dealt in units of a step's time; an item's change of Q, output or partial and first scores, in which the
-// tensor core idles, count as kItemUnits more in front of its steps.
+// The list is dealt in units of a step's time; an item's output or partial and its first softmax, in which the
+// tensor core idles, count as kItemUnits more in front of its steps. (Without them the CTAs with the shortest items end
+// last: half as much time again for a ragged batch.)
 constexpr int kItemUnits = 4;
-constexpr int kMinShare = 8;  // units of a CTA at least
+// Units of a CTA at least. Two short tails on 300 to 700 tokens take 13.9 us with 4; 8 and 12 cost 3.7 and 7 us more: the
+// join costs less than a step or two.
+constexpr int kMinShare = 4;
 constexpr int kPartRows = 2 * kRows;
 constexpr int kPartFloats = kPartRows * (kD + 2);  // O as [32 x 4 elements][row][4], then (reference, sum) per row
 
@@ -244,6 +271,13 @@ struct Cursor {
     own_steps(count);
     return true;
   }
+};
+
+// What a tile's softmax warps need to know of an item; written by the warp that issues the tile's products.
+struct Item {
+  int seq, kvh, q0, n_tok;         // q0: row of q of the item's first token, n_tok: its tokens
+  int pos, kv_len, key_end;        // pos: position of the first token, key_end: end of the keys of this CTA's steps
+  int j0, j1, whole;               // this CTA's steps, and whether they are all of them
 };
 
 // The 16-element groups in which V has a NaN among keys [k0, k1) up to `lim` of the calling lane's row, a
@@ -359,9 +393,11 @@ __device__ __forceinline__ int find_share(const PrefillArgs& a, Cursor& c, int64
   return c.j0 < c.j1 || c.next_item(a, count) ? count : 0;
 }
 
-__global__ void __launch_bounds__(kThreads, 1) prefill_fp4_kernel(const __grid_constant__ PrefillArgs a) {
+__global__ void __launch_bounds__(kThreads, 1)
+    prefill_fp4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ PrefillArgs a) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
-  __shared__ uint64_t q_full[2], full[kSlots], empty[kSlots], s_full[2][2], p_ready[2][2], pv_done[2][2];
+  __shared__ uint64_t q_full[2], full[kSlots], empty[kSlots], s_full[2][2], p_ready[2][2], pv_done[2][2], item_full[2];
+  __shared__ Item s_item[2][2];  // per tile, the item at hand and the one behind it
   __shared__ uint32_t s_tmem;
   __shared__ Cursor s_first;
   __shared__ int s_count;
@@ -396,7 +432,8 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_fp4_kernel(const __grid_c
         mbar_init(&empty[i], 2);  // both tiles' warps are done with the slot
       }
       for (int i = 0; i < 2; ++i) {
-        mbar_init(&q_full[i], 128);
+        mbar_init(&q_full[i], 1);
+        mbar_init(&item_full[i], 1);
         for (int h = 0; h < 2; ++h) {  // the steps' parities
           mbar_init(&s_full[i][h], 1);
           mbar_init(&p_ready[i][h], 128);
@@ -421,49 +458,16 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_fp4_kernel(const __grid_c
     // ------------------------------------------------------------------ softmax
     const int t = warp >> 2;                        // tile
     const int row = (warp & 3) * 32 + lane;         // TMEM lane
-    const int tt = t * tpt + row / G, h = row % G;  // token of the item, head of the group
+    const int tt = t * tpt + ((row * a.inv_g) >> 16);  // token of the item
     const uint32_t lane_base = tmem + ((uint32_t)((warp & 3) * 32) << 16);
     const uint32_t o_addr = lane_base + kColO + t * kD;
     int js = 0;  // steps of this tile so far: the barriers' phases
-    // the item at hand or the next one behind it that has rows in this tile
-    auto find = [&](bool more) {
-      for (; more; more = cu.next_item(a, count)) {
-        if (threadIdx.x == 0 && cu.j0 == 0 && cu.j1 < cu.steps)
-          a.open_items[blockIdx.x] = make_int4((int)((cu.end() - count + s_share - 1) / s_share), cu.s, cu.b, cu.h);
-        if (t * tpt < cu.q.q_len - cu.b * a.tok) return true;
-      }
-      return false;
-    };
-    auto fetch_q = [&] {  // 16 lanes a row
-      const int tw = threadIdx.x & 127, ch = tw & 15, tok0 = cu.b * a.tok;
-      const uint32_t dst = smem_u32(s_q) + (t * 2 + (ch >> 3)) * kQHalf;
-      const __half* src = a.q + (int64_t)(cu.q.q_start + tok0) * a.q_ts + cu.h * G * kD + ch * 8;
-#pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int r = (tw >> 4) + 8 * i, rt = (r * a.inv_g) >> 16;  // token of the tile
-        const int qt = t * tpt + rt;
-        const bool in = rt < tpt && qt < min(a.tok, cu.q.q_len - tok0);
-        cp_async16_zfill(dst + r * 128 + (((ch & 7) ^ (r & 7)) << 4), in ? src + qt * a.q_ts + (r - rt * G) * kD : a.q, in);
-      }
-    };
-    auto hand_q = [&] {
-      cp_async_wait_all();
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      mbar_arrive(&q_full[t]);
-    };
-    bool more = find(count > 0);
-    if (more) {
-      fetch_q();
-      hand_q();
-    }
-    while (more) {
-      const int j0 = cu.j0, j1 = cu.j1;
-      const bool whole = j0 == 0 && j1 == cu.steps;
-      const int tok0 = cu.b * a.tok, n_tok = min(a.tok, cu.q.q_len - tok0);
-      const bool valid = row < tpt * G && tt < n_tok;
-      const int lim = valid ? min(cu.q.prefix + tok0 + tt, cu.q.kv_len - 1) : -1;  // last visible key
-      const int seq = cu.s, kvh = cu.h, seen_end = min(j1 * kKeys, cu.keys);
-      const int64_t out_row = ((int64_t)(cu.q.q_start + tok0 + tt) * a.Hkv + kvh) * G + h;
+    for (int it = 0; warp_wait(&item_full[t], it & 1); ++it) {
+      // read where it is needed: the loop over the steps has no registers to spare
+      const volatile Item& item = s_item[t][it & 1];
+      const int j0 = item.j0, j1 = item.j1;
+      if (j0 == j1) break;  // behind the last item
+      const int lim = row < tpt * G && tt < item.n_tok ? min(item.pos + tt, item.kv_len - 1) : -1;  // last visible key
       int low = lim;  // smallest limit of the warp: steps below it need no mask
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) low = min(low, __shfl_xor_sync(0xffffffffu, low, o));
@@ -488,7 +492,7 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_fp4_kernel(const __grid_c
             uint32_t seen = n >= 32 ? 0xffffffffu : (n <= 0 ? 0u : (1u << n) - 1u);
             if (bad) {  // rare: leave out the keys of bad pages
               const int pg = k0 / a.block_size;
-              const int64_t blk = pg < a.max_blocks ? a.tables[(int64_t)seq * a.max_blocks + pg] : -1;
+              const int64_t blk = pg < a.max_blocks ? a.tables[(int64_t)item.seq * a.max_blocks + pg] : -1;
               if (blk < 0 || blk >= a.num_blocks) seen = 0;
             }
             hide(v[c], seen);
@@ -546,41 +550,47 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_fp4_kernel(const __grid_c
         l += x0 + x1;
       }
       if (!ok) break;
-      // Q is no longer read: fetch the next item's under the last product, so that its first scores are made
-      // under this item's end
-      more = find(cu.next_item(a, count));
-      if (more) fetch_q();
       // The last product. S of its step was issued before the product of step js - 2, which may still run,
       // hence a barrier per parity of steps: one for both could not tell the two by its phase.
       ok = warp_wait(&pv_done[t][(js - 1) & 1], ((js - 1) >> 1) & 1);
-      if (more) hand_q();
       if (!ok) break;
       tc_fence_after();
       // ---- the item's steps of this CTA are done: O / l, or a partial ------------------------------
       uint32_t nan = 0;  // 16-element groups in which this row sees a NaN of V
       if (__any_sync(0xffffffffu, *reinterpret_cast<volatile int*>(&s_seen_nan) != 0))
-        nan = nan_groups(a, seq, kvh, j0 * kKeys, seen_end, lim);
+        nan = nan_groups(a, item.seq, item.kvh, item.j0 * kKeys, item.key_end, lim);
       const float qnan = __int_as_float(0x7fffffff);
-      if (whole) {
+      if (item.whole) {
         const float inv = l == 0.f ? 0.f : 1.f / l;
-        __half* dst = a.out + out_row * kD;
+        // four lanes store 64 bytes of a row: 8 lines an instruction, where a row a lane would take 32
+        const int n_tok = item.n_tok, q0 = item.q0, kvh = item.kvh;
+        __half* dst[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const int r = (row & ~3) + i, rt = (r * a.inv_g) >> 16, tok = t * tpt + rt;
+          dst[i] = rt < tpt && tok < n_tok
+                       ? a.out + ((((int64_t)(q0 + tok) * a.Hkv + kvh) * G + (r - rt * G)) * kD + (lane & 3) * 8)
+                       : nullptr;
+        }
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           float o[32];
+          uint32_t p[16];
           tmem_ld32(o_addr + 32 * c, o);
           tmem_ld_wait();
-          if (valid) {
 #pragma unroll
-            for (int i = 0; i < 32; i += 8) {
-              const float f = (nan >> (2 * c + (i >> 4))) & 1u ? qnan : inv;
-              *reinterpret_cast<uint4*>(dst + 32 * c + i) =
-                  make_uint4(pack_h2(o[i] * f, o[i + 1] * f), pack_h2(o[i + 2] * f, o[i + 3] * f),
-                             pack_h2(o[i + 4] * f, o[i + 5] * f), pack_h2(o[i + 6] * f, o[i + 7] * f));
-            }
+          for (int i = 0; i < 32; i += 2) {
+            const float f = (nan >> (2 * c + (i >> 4))) & 1u ? qnan : inv;
+            p[i >> 1] = pack_h2(o[i] * f, o[i + 1] * f);
           }
+          transpose4(p);
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (dst[i] != nullptr)
+              *reinterpret_cast<uint4*>(dst[i] + 32 * c) = make_uint4(p[4 * i], p[4 * i + 1], p[4 * i + 2], p[4 * i + 3]);
         }
       } else {  // slot 0: the item began in an earlier CTA; slot 1: it begins here and goes on
-        float* part = a.ws + ((int64_t)blockIdx.x * 2 + (j0 > 0 ? 0 : 1)) * kPartFloats;
+        float* part = a.ws + ((int64_t)blockIdx.x * 2 + (item.j0 > 0 ? 0 : 1)) * kPartFloats;
         const int pr = t * kRows + row;
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
@@ -706,9 +716,28 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_fp4_kernel(const __grid_c
     };
     int js = 0, items = 0;
     bool ok = true;
-    for (bool more = count > 0; more; more = cu.next_item(a, count)) {
-      const int j0 = cu.j0, j1 = cu.j1;
-      if (t * tpt >= min(a.tok, cu.q.q_len - cu.b * a.tok)) {  // no rows in this tile: pass the slots on
+    bool more = count > 0;
+    while (more) {
+      const int j0 = cu.j0, j1 = cu.j1, tok0 = cu.b * a.tok;
+      const bool rows = t * tpt < cu.q.q_len - tok0;
+      if (rows && lead) {
+        if (t == 0 && j0 == 0 && j1 < cu.steps)
+          a.open_items[blockIdx.x] = make_int4((int)((cu.end() - count + s_share - 1) / s_share), cu.s, cu.b, cu.h);
+        // the buffer's last item was the one before the last: its softmax is over, since the last one's steps are
+        s_item[t][items & 1] = Item{cu.s, cu.h, cu.q.q_start + tok0, min(a.tok, cu.q.q_len - tok0),
+                                    cu.q.prefix + tok0, cu.q.kv_len, min(j1 * kKeys, cu.keys),
+                                    j0, j1, j0 == 0 && j1 == cu.steps};
+        mbar_arrive(&item_full[t]);
+        // Q was last read for the scores whose weights have been waited for. The box has rows (token, head), also of
+        // tokens behind the item's
+        mbar_arrive_expect_tx(&q_full[t], 2 * tpt * G * 128);
+        for (int i = 0; i < 2; ++i)
+          tma_load_3d(&tmap_q, smem_u32(s_q) + (t * 2 + i) * kQHalf, &q_full[t], i * 64, cu.h * G,
+                      cu.q.q_start + tok0 + t * tpt);
+      }
+      __syncwarp();
+      more = cu.next_item(a, count);  // from here on `cu` is the next item
+      if (!rows) {  // pass the slots on
         for (int j = j0; ok && j < j1; ++j) {
           ok = warp_wait(&full[k.stage], k.par);
           if (ok) release(k);
@@ -746,6 +775,11 @@ __global__ void __launch_bounds__(kThreads, 1) prefill_fp4_kernel(const __grid_c
       }
       if (!ok) break;
     }
+    if (lead) {
+      s_item[t][items & 1].j0 = s_item[t][items & 1].j1 = 0;
+      mbar_arrive(&item_full[t]);
+    }
+    __syncwarp();
     // no arrival may outlive the CTA: wait for the release of each slot's last use (the places point behind it)
     for (int i = 0; ok && i < kSlots; ++i) {
       const Place& p = (i & 1) ? v : k;
@@ -829,8 +863,6 @@ cudaError_t launch_prefill_fp4(const void* q, int64_t q_ts, const void* k_cache,
                                int num_seqs, int total_q, int Hq, int Hkv, int block_size, int max_blocks,
                                float softmax_scale, void* workspace, int num_sms, cudaStream_t stream) {
   PrefillArgs a = {};
-  a.q = (const __half*)q;
-  a.q_ts = q_ts;
   a.kc = (const uint8_t*)k_cache;
   a.vc = (const uint8_t*)v_cache;
   a.ks = (const uint8_t*)k_scale;
@@ -864,7 +896,18 @@ cudaError_t launch_prefill_fp4(const void* q, int64_t q_ts, const void* k_cache,
     attr = cudaFuncSetAttribute(prefill_fp4_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
   });
   if (attr != cudaSuccess) return attr;
-  const cudaError_t e = launch_kernel(prefill_fp4_kernel, dim3(ctas), dim3(kThreads), kSmemBytes, stream, a);
+  // Q as (element, head, token); a box is 64 elements of a tile's rows
+  const EncodeTiledFn encode = get_encode_fn();
+  if (encode == nullptr) return cudaErrorNotSupported;
+  CUtensorMap map;
+  const cuuint64_t dims[3] = {(cuuint64_t)kD, (cuuint64_t)Hq, (cuuint64_t)total_q};
+  const cuuint64_t strides[2] = {(cuuint64_t)kD * 2, (cuuint64_t)q_ts * 2};
+  const cuuint32_t box[3] = {64, (cuuint32_t)a.G, (cuuint32_t)(kRows / a.G)}, step[3] = {1, 1, 1};
+  if (encode(&map, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(q), dims, strides, box, step,
+             CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+             CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+    return cudaErrorInvalidValue;
+  const cudaError_t e = launch_kernel(prefill_fp4_kernel, dim3(ctas), dim3(kThreads), kSmemBytes, stream, map, a);
   if (e != cudaSuccess || ctas == 1) return e;
   return launch_kernel(merge_prefill_fp4_kernel, dim3(ctas - 1, kPartRows / 32), dim3(kMergeThreads), 0, stream, a);
 }

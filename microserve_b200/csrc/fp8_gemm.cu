@@ -39,6 +39,7 @@
 
 #include "common.cuh"
 #include "kernels.h"
+#include "tensor_map.h"
 #include "tp_rows.cuh"
 
 namespace ms {
@@ -1162,23 +1163,6 @@ __global__ void fp8_gemm_simt_kernel(const uint8_t* __restrict__ xq, const uint8
 // ---------------------------------------------------------------------------
 // Host side: tensor-map encoding (driver entry point, cached), tile choice.
 // ---------------------------------------------------------------------------
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                  const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                  CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-EncodeTiledFn get_encode_fn() {
-  static EncodeTiledFn fn = nullptr;
-  static std::once_flag once;
-  std::call_once(once, [] {
-    void* p = nullptr;
-    cudaDriverEntryPointQueryResult q;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
-        q == cudaDriverEntryPointSuccess)
-      fn = reinterpret_cast<EncodeTiledFn>(p);
-  });
-  return fn;
-}
-
 struct MapKey {
   const void* ptr;
   int64_t rows, cols;
