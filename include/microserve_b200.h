@@ -240,7 +240,8 @@ int ms_paged_decode_fp4(const void* q, int64_t q_token_stride, const void* k_cac
  * q[cu_q[s] .. cu_q[s+1]) at positions kv_lens[s] - q_len_s + i, each seeing the keys
  * up to its own position (none below position 0: output 0). Rows of out behind
  * cu_q[num_seqs] are not written, offsets outside [0, total_q] are cut. Workspace as for
- * ms_paged_decode_fp4. */
+ * ms_paged_decode_fp4. Refused where (total_q * Hq / Hkv / 256 + num_seqs) * Hkv *
+ * (max_blocks * block_size / 64) comes near 2^31 (steps are counted in 32 bits). */
 size_t ms_paged_prefill_fp4_workspace_size(int num_seqs, int64_t total_q, int Hq, int Hkv, int max_blocks,
                                            int block_size);
 int ms_paged_prefill_fp4(const void* q, int64_t q_token_stride, const void* k_cache, const void* v_cache,

@@ -68,6 +68,19 @@ __device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.lau
 extern std::atomic<int> g_pdl_enabled;
 extern std::atomic<int> g_pair_tiles_enabled;  // FP8/fp16 GEMM: SM-pair schedules allowed
 
+// Opt `kernel` in to `bytes` of dynamic shared memory, once per device (`done`: a static of the call site).
+template <typename... KArgs>
+cudaError_t allow_smem(void (*kernel)(KArgs...), int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = dev < 64 ? (uint64_t)1 << dev : 0;
+  if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+  e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+  if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+  return e;
+}
+
 template <typename... KArgs, typename... Args>
 cudaError_t launch_kernel(void (*kernel)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t stream,
                           Args&&... args) {

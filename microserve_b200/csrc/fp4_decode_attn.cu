@@ -29,8 +29,6 @@
 //    product as two f16 parts (hi + lo, scaled by 2^10: at most 2^15), so outputs keep
 //    fp32-level accuracy; with G <= 4 both parts share one MMA (columns 0-3 hi, 4-7 lo),
 //    with more heads it takes two.
-#include <mutex>
-
 #include "fp4_kv.cuh"
 #include "kernels.h"
 
@@ -702,16 +700,12 @@ cudaError_t launch_decode_fp4(const void* q, int64_t q_ts, const void* k_cache, 
   a.open_items = (int4*)workspace;
   a.ws = (float*)((int4*)workspace + ctas);
   const bool two = a.G > 4;
-  static std::once_flag once;
-  static cudaError_t attr = cudaSuccess;
-  std::call_once(once, [] {
-    attr = cudaFuncSetAttribute(decode_fp4_kernel<false>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(4));
-    if (attr == cudaSuccess)
-      attr = cudaFuncSetAttribute(decode_fp4_kernel<true>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem_bytes(8));
-  });
-  if (attr != cudaSuccess) return attr;
-  cudaError_t e = two ? launch_kernel(decode_fp4_kernel<true>, dim3(ctas), dim3(kThreads), smem_bytes(8), stream, a)
-                      : launch_kernel(decode_fp4_kernel<false>, dim3(ctas), dim3(kThreads), smem_bytes(4), stream, a);
+  static std::atomic<uint64_t> allowed[2];
+  cudaError_t e = two ? allow_smem(decode_fp4_kernel<true>, smem_bytes(8), allowed[1])
+                      : allow_smem(decode_fp4_kernel<false>, smem_bytes(4), allowed[0]);
+  if (e != cudaSuccess) return e;
+  e = two ? launch_kernel(decode_fp4_kernel<true>, dim3(ctas), dim3(kThreads), smem_bytes(8), stream, a)
+          : launch_kernel(decode_fp4_kernel<false>, dim3(ctas), dim3(kThreads), smem_bytes(4), stream, a);
   if (e != cudaSuccess || ctas == 1) return e;
   return launch_kernel(merge_fp4_kernel, dim3(ctas - 1), dim3(kMergeThreads), 0, stream, a);
 }

@@ -36,8 +36,6 @@
 // of V as zeros too, because a zero weight does not hide a NaN from the product; where one was
 // met, the first key with a NaN is looked up per 16 elements at the end of the item, and the rows
 // that see it get NaN.
-#include <mutex>
-
 #include "fp4_kv.cuh"
 #include "kernels.h"
 #include "tensor_map.h"
@@ -890,12 +888,9 @@ cudaError_t launch_prefill_fp4(const void* q, int64_t q_ts, const void* k_cache,
   const int ctas = prefill_fp4_ctas(num_seqs, total_q, Hkv, a.G, max_blocks, block_size, num_sms);
   a.open_items = (int4*)workspace;
   a.ws = (float*)((int4*)workspace + ctas);
-  static std::once_flag once;
-  static cudaError_t attr = cudaSuccess;
-  std::call_once(once, [] {
-    attr = cudaFuncSetAttribute(prefill_fp4_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmemBytes);
-  });
-  if (attr != cudaSuccess) return attr;
+  static std::atomic<uint64_t> allowed{0};
+  cudaError_t e = allow_smem(prefill_fp4_kernel, kSmemBytes, allowed);
+  if (e != cudaSuccess) return e;
   // Q as (element, head, token); a box is 64 elements of a tile's rows
   const EncodeTiledFn encode = get_encode_fn();
   if (encode == nullptr) return cudaErrorNotSupported;
@@ -907,7 +902,7 @@ cudaError_t launch_prefill_fp4(const void* q, int64_t q_ts, const void* k_cache,
              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
     return cudaErrorInvalidValue;
-  const cudaError_t e = launch_kernel(prefill_fp4_kernel, dim3(ctas), dim3(kThreads), kSmemBytes, stream, map, a);
+  e = launch_kernel(prefill_fp4_kernel, dim3(ctas), dim3(kThreads), kSmemBytes, stream, map, a);
   if (e != cudaSuccess || ctas == 1) return e;
   return launch_kernel(merge_prefill_fp4_kernel, dim3(ctas - 1, kPartRows / 32), dim3(kMergeThreads), 0, stream, a);
 }
