@@ -6,6 +6,7 @@ Every function requires CUDA tensors; there is no CPU path.
 """
 from __future__ import annotations
 
+import functools
 import threading
 
 import torch
@@ -417,6 +418,17 @@ def _int32(what: str, name: str, t: torch.Tensor, *shape: int) -> None:
                      f"[{', '.join('*' if s < 0 else str(s) for s in shape)}]")
 
 
+# Workspace bytes by sizes (and device: its SMs), looked up once: the C call takes a third of a launch.
+@functools.lru_cache(maxsize=1024)
+def _decode_fp4_workspace(device: int, *sizes: int) -> int:
+    return _lib.load().ms_paged_decode_fp4_workspace_size(*sizes)
+
+
+@functools.lru_cache(maxsize=1024)
+def _prefill_fp4_workspace(device: int, *sizes: int) -> int:
+    return _lib.load().ms_paged_prefill_fp4_workspace_size(*sizes)
+
+
 def paged_decode_fp4(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Tensor,
                      v_scale: torch.Tensor, cache_seqlens: torch.Tensor, block_tables: torch.Tensor,
                      softmax_scale: float, out: torch.Tensor | None = None) -> torch.Tensor:
@@ -428,15 +440,13 @@ def paged_decode_fp4(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.
     _int32("paged_decode_fp4", "block_tables", block_tables, B, -1)
     query, q_stride, o = _fp4_query("paged_decode_fp4", query, out)
     _on_current_device("paged_decode_fp4", query, k_cache, v_cache, k_scale, v_scale, cache_seqlens, block_tables, o)
-    lib = _lib.load()
     max_blocks = block_tables.shape[1]
     # a workspace of its own for every call: calls on two streams, or two captured graphs, never share one
-    ws = torch.empty(lib.ms_paged_decode_fp4_workspace_size(B, Hq, Hkv, max_blocks, BS), dtype=torch.uint8,
-                     device=query.device)
-    check(lib.ms_paged_decode_fp4(query.data_ptr(), q_stride, k_cache.data_ptr(), v_cache.data_ptr(),
-                                  k_scale.data_ptr(), v_scale.data_ptr(), NB, cache_seqlens.data_ptr(),
-                                  block_tables.data_ptr(), o.data_ptr(), B, Hq, Hkv, D, BS, max_blocks,
-                                  float(softmax_scale), ws.data_ptr(), ws.numel(), stream_ptr()),
+    ws = k_cache.new_empty(_decode_fp4_workspace(o.get_device(), B, Hq, Hkv, max_blocks, BS))
+    check(_lib.load().ms_paged_decode_fp4(query.data_ptr(), q_stride, k_cache.data_ptr(), v_cache.data_ptr(),
+                                          k_scale.data_ptr(), v_scale.data_ptr(), NB, cache_seqlens.data_ptr(),
+                                          block_tables.data_ptr(), o.data_ptr(), B, Hq, Hkv, D, BS, max_blocks,
+                                          float(softmax_scale), ws.data_ptr(), ws.numel(), stream_ptr()),
           "ms_paged_decode_fp4")
     return o
 
@@ -455,14 +465,14 @@ def paged_prefill_fp4(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     _int32("paged_prefill_fp4", "block_tables", block_tables, num_seqs, -1)
     query, q_stride, o = _fp4_query("paged_prefill_fp4", query, out)
     _on_current_device("paged_prefill_fp4", query, k_cache, v_cache, k_scale, v_scale, block_tables, cu_q, kv_lens, o)
-    lib = _lib.load()
     max_blocks = block_tables.shape[1]
-    ws = torch.empty(lib.ms_paged_prefill_fp4_workspace_size(num_seqs, T, Hq, Hkv, max_blocks, BS), dtype=torch.uint8,
-                     device=query.device)  # its own for every call, as in paged_decode_fp4
-    check(lib.ms_paged_prefill_fp4(query.data_ptr(), q_stride, k_cache.data_ptr(), v_cache.data_ptr(),
-                                   k_scale.data_ptr(), v_scale.data_ptr(), NB, block_tables.data_ptr(),
-                                   cu_q.data_ptr(), kv_lens.data_ptr(), o.data_ptr(), num_seqs, T, Hq, Hkv, D, BS,
-                                   max_blocks, float(softmax_scale), ws.data_ptr(), ws.numel(), stream_ptr()),
+    # its own for every call, as in paged_decode_fp4
+    ws = k_cache.new_empty(_prefill_fp4_workspace(o.get_device(), num_seqs, T, Hq, Hkv, max_blocks, BS))
+    check(_lib.load().ms_paged_prefill_fp4(query.data_ptr(), q_stride, k_cache.data_ptr(), v_cache.data_ptr(),
+                                           k_scale.data_ptr(), v_scale.data_ptr(), NB, block_tables.data_ptr(),
+                                           cu_q.data_ptr(), kv_lens.data_ptr(), o.data_ptr(), num_seqs, T, Hq, Hkv,
+                                           D, BS, max_blocks, float(softmax_scale), ws.data_ptr(), ws.numel(),
+                                           stream_ptr()),
           "ms_paged_prefill_fp4")
     return o
 
