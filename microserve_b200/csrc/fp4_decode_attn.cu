@@ -5,8 +5,9 @@
 // Bound by the cache's bytes (144 per token and kv head) and, close behind, by the
 // instructions that turn 4-bit codes into f16 operands, so both are kept even and few.
 // 241 MB of cache (256 sequences of 128 to 1536 tokens, 32 / 8 heads) take 61 us, 0.61 of the copy bandwidth:
-// tiles stream at 0.93 of it, and 15 us go to the scan and page look-ups (4 to 5), the CTAs' uneven ends,
-// the joins and the second kernel.
+// 4.5 us to the first tile (scan, page look-up, copy: three memory latencies), 46 to 53 for an SM's tiles (its
+// copies alone 44, its arithmetic alone 54 with the overheads: 640 instructions a tile and warp at 0.54 a cycle and
+// scheduler), 3 for the join, 2.5 for the second kernel.
 //  * The work is one flat list of 32-token tiles over (sequence, kv head, tile). The grid
 //    fills the SMs once; every CTA takes an equal contiguous share of the list (found by
 //    a scan of seqlens) and every warp a quarter of that, whatever the lengths are. A warp
