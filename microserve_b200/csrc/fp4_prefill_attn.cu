@@ -8,7 +8,7 @@
 // keys that both tiles read. The steps of all items (sequence, block of tokens, kv head) form
 // one list that is dealt evenly to one CTA per SM, whatever the lengths are; an item that
 // crosses CTAs leaves fp32 partials (O, reference, sum) in the workspace, joined by a second kernel.
-// 2048 queries behind 30720 tokens (32 / 8 heads) take 997 us, 1068 TFLOP/s of visible pairs.
+// 2048 queries behind 30720 tokens (32 / 8 heads) take 1010 us, 1055 TFLOP/s of visible pairs.
 // The roles below walk a CTA's items on their own, so decoding runs ahead into the next one.
 //   warps 0-3, 4-7   softmax of tile 0 / 1: a thread owns a row. It reads its 64 scores of a
 //                    step from TMEM, writes the weights over them as f16, and keeps the row's
@@ -29,8 +29,9 @@
 // chain's latencies show, 4 and 16 % more time.
 // Softmax in the exp2 domain against a lazy reference: weights are 2^(s - m) for a reference
 // m that moves, with a rescale of O in TMEM, only when a row's maximum exceeds it by 8 or
-// more. Weights are rounded to f16 for the second product (2^-11 relative; the first
-// rounding below fp32 in the kernel, K and V are exact), the row sums take them unrounded.
+// more. Weights are rounded to f16 for the second product (2^-11 relative, 2^-31 of the largest
+// where they are subnormal; the first rounding below fp32 in the kernel, K and V are exact), the
+// row sums take them unrounded.
 //
 // V rows behind an item's last key and rows of bad pages are written as zeros, and a NaN group
 // of V as zeros too, because a zero weight does not hide a NaN from the product; where one was
