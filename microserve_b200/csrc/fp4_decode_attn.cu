@@ -4,14 +4,14 @@
 //
 // Bound by the cache's bytes (144 per token and kv head) and, close behind, by the
 // instructions that turn 4-bit codes into f16 operands, so both are kept even and few.
-// 241 MB of cache (256 sequences of 128 to 1536 tokens, 32 / 8 heads) take 61 us, 0.61 of the copy bandwidth:
-// 4.5 us to the first tile (scan, page look-up, copy: three memory latencies), 46 to 53 for an SM's tiles (its
+// 241 MB of cache (256 sequences of 128 to 1536 tokens, 32 / 8 heads) take 58 us, 0.64 of the copy bandwidth:
+// 4.5 us to the first tile (scan, page look-up, copy: three memory latencies), 46 to 50 for an SM's tiles (its
 // copies alone 44, its arithmetic alone 54 with the overheads: 640 instructions a tile and warp at 0.54 a cycle and
 // scheduler), 3 for the join, 2.5 for the second kernel.
 //  * The work is one flat list of 32-token tiles over (sequence, kv head, tile). The grid
-//    fills the SMs once; every CTA takes an equal contiguous share of the list (found by
-//    a scan of seqlens) and every warp a quarter of that, whatever the lengths are. A warp
-//    keeps kStages tiles (codes and scales of K and V) in flight through its own ring
+//    fills the SMs once; every CTA takes an equal contiguous share of the list, an item's own
+//    cost counted like a tile (found by a scan of seqlens), and every warp a quarter of that,
+//    whatever the lengths are. A warp keeps kStages tiles (codes and scales of K and V) in flight through its own ring
 //    of shared memory (cp.async), across the borders of items (sequence, kv head). An item
 //    inside one warp's share is finished by that warp alone; the pieces of one that
 //    crosses warps are joined in shared memory at the end of the CTA, of one that crosses
@@ -47,7 +47,10 @@ constexpr int kStageBytes = 2 * kCodeBytes + 2 * kScBytes;
 constexpr int kRingBytes = kWarps * kStages * kStageBytes;
 constexpr int kRowFloats = kD + 4;         // a partial of one head in shared memory: o[128], m, l, padding
 constexpr int kCtasPerSm = 3;
-constexpr int kMinShare = 4;               // tiles of a CTA at least: one a warp (one sequence of 300: 7.9 us, 8.8 with two)
+// The list is dealt in units of a tile's time: an item's first load of Q, sums over lanes and output count as
+// kItemUnits behind its tiles (256 sequences of 128 to 1536 tokens: 60.5 us without, 58.0 with 1, 58.4 with 2).
+constexpr int kItemUnits = 1;
+constexpr int kMinShare = 4;               // units of a CTA at least: one a warp (one sequence of 300: 7.9 us, 8.8 with two)
 constexpr int kPartFloats = kD + 2;        // a partial of one head: o[128], m, l
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr float kPScaleLog2 = 10.f;        // weights are scaled by 2^10: lo stays a normal f16 where it matters,
@@ -115,11 +118,12 @@ struct DecodeArgs {
 // Tokens of sequence b (0 where negative, cut at the table's end) and its tiles.
 __device__ __forceinline__ int seq_len(const DecodeArgs& a, int b) { return min(max(a.seqlens[b], 0), a.cap); }
 __device__ __forceinline__ int tiles_of(int len) { return (len + kTile - 1) / kTile; }
+__device__ __forceinline__ int units_of(int nt) { return nt > 0 ? nt + kItemUnits : 0; }  // of an item of nt tiles
 
-// The flat tile list: the tiles of a kv head in all sequences before the calling thread's own,
+// The flat tile list: the units of a kv head in all sequences before the calling thread's own,
 // [b0, b1), and in all of them. Whole block.
 struct Scan {
-  int64_t before, total;  // in tiles of one kv head
+  int64_t before, total;  // in units of one kv head
   int b0, b1;
 };
 __device__ __forceinline__ Scan scan_lens(const DecodeArgs& a, int64_t* red) {
@@ -128,7 +132,7 @@ __device__ __forceinline__ Scan scan_lens(const DecodeArgs& a, int64_t* red) {
   s.b0 = min((int)threadIdx.x * per, a.B);
   s.b1 = min(s.b0 + per, a.B);
   int64_t mine = 0;
-  for (int b = s.b0; b < s.b1; ++b) mine += tiles_of(seq_len(a, b));
+  for (int b = s.b0; b < s.b1; ++b) mine += units_of(tiles_of(seq_len(a, b)));
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int64_t inc = mine;
 #pragma unroll
@@ -147,18 +151,18 @@ __device__ __forceinline__ Scan scan_lens(const DecodeArgs& a, int64_t* red) {
   }
   return s;
 }
-// Tiles a CTA takes.
+// Units a CTA takes.
 __device__ __forceinline__ int64_t share_of(int64_t total, int ctas) {
   const int64_t even = (total + ctas - 1) / ctas;
   return even > kMinShare ? even : kMinShare;
 }
 
-// Position in the CTA's tiles: item (b, h) of nt tiles and len tokens starts at relative
-// tile `start` (negative: in an earlier CTA).
+// Position in a warp's units: item (b, h) of nt tiles and len tokens starts at relative
+// unit `start` (negative: in an earlier warp).
 struct Cursor {
   int b, h, nt, len, start;
   __device__ __forceinline__ void next_item(const DecodeArgs& a) {
-    start += nt;
+    start += nt + kItemUnits;
     if (++h == a.Hkv) {
       h = 0;
       do {
@@ -208,26 +212,26 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_fp4_kernel(const 
     if (threadIdx.x == 0) a.open_items[blockIdx.x] = make_int4(0, 0, 0, 0);
     return;
   }
-  const int cta_tiles = (int)(total - begin < share ? total - begin : share);
-  auto warp_begin = [&](int w) { return (int)((int64_t)cta_tiles * w / kWarps); };
+  const int cta_units = (int)(total - begin < share ? total - begin : share);
+  auto warp_begin = [&](int w) { return (int)((int64_t)cta_units * w / kWarps); };
   {  // the threads whose sequences hold the warps' first tiles leave their items
     int64_t at = sc.before * a.Hkv;
     for (int b = sc.b0; b < sc.b1; ++b) {
-      const int len = seq_len(a, b), nt = tiles_of(len);
-      const int64_t end = at + (int64_t)nt * a.Hkv;
+      const int len = seq_len(a, b), nt = tiles_of(len), nu = units_of(nt);
+      const int64_t end = at + (int64_t)nu * a.Hkv;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         const int64_t x = begin + warp_begin(w);
         if (x >= at && x < end) {
-          const int h = (int)((x - at) / nt);
-          s_first[w] = Cursor{b, h, nt, len, -(int)(x - at - (int64_t)h * nt)};
+          const int h = (int)((x - at) / nu);
+          s_first[w] = Cursor{b, h, nt, len, -(int)(x - at - (int64_t)h * nu)};
         }
       }
       at = end;
     }
   }
   __syncthreads();
-  const int count = warp_begin(warp + 1) - warp_begin(warp);  // tiles of this warp
+  const int count = warp_begin(warp + 1) - warp_begin(warp);  // units of this warp
 
   // ---- this warp's ring --------------------------------------------------------------
   unsigned char* ring = smem + warp * (kStages * kStageBytes);
@@ -241,13 +245,19 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_fp4_kernel(const 
     const int q = lane + 32 * i, tok = q >> 2, j = q & 3;
     v_dst[i] = (uint32_t)(kCodeBytes + ((tok ^ ((tok >> 4) & 1)) * kFp4RowBytes) + ((j ^ (((tok >> 3) & 1) << 1)) << 4));
   }
-  Cursor is = s_first[warp];  // issue side: the item of tile is_r
-  int is_r = 0;
+  Cursor cu = s_first[warp];
+  if (count > 0 && cu.start + cu.nt <= 0) cu.next_item(a);  // the share begins behind the item's tiles
+  Cursor is = cu;  // issue side: the item of tile is_r
+  int is_r = max(is.start, 0);
   uint32_t bad = 0;     // stages whose tile has no valid page
   int64_t is_row = 0;   // first cache row of tile is_r, -1: none
   int page_left = 0;    // tiles left in its page, this one included
   auto look_up = [&] {  // the page of tile is_r
-    if (is_r == is.start + is.nt) is.next_item(a);
+    if (is_r == is.start + is.nt) {
+      is.next_item(a);
+      is_r = is.start;
+      if (is_r >= count) return;
+    }
     const int p0 = (is_r - is.start) * kTile;
     const int page = a.bs_log2 >= 0 ? p0 >> a.bs_log2 : p0 / a.block_size;
     const int off = p0 - page * a.block_size;
@@ -279,7 +289,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_fp4_kernel(const 
     }
     cp_async_commit();  // one group per slot, empty or not
   };
-  if (count > 0) look_up();
+  if (is_r < count) look_up();
 #pragma unroll
   for (int k = 0; k < kStages; ++k) issue(k);
 
@@ -288,10 +298,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_fp4_kernel(const 
   const uint32_t v_odd = (uint32_t)((8 * c + 1 - (c >> 1)) * kFp4RowBytes + (((g >> 1) ^ ((c & 1) << 1)) << 4) + (g & 1) * 8);
   const int tok_a = 8 * (g >> 1) + (g & 1);  // token of MMA row g: tok_a + 4 tile + 2 (row >= 8)
 
-  Cursor cu = s_first[warp];
   Pieces pieces = {0, 0, 0, 0, 0, 0, 0, 0};
-  int r = 0, slot = 0;
-  while (r < count) {
+  int r = max(cu.start, 0), slot = 0;
+  while (r < count && cu.b < a.B) {  // (behind the last sequence: only if seqlens changed meanwhile)
     const int seg_end = min(cu.start + cu.nt, count);
     // Q fragment: column g = head g (G <= 4: columns 4-7 repeat 0-3), d = 32 c + [0, 32)
     uint32_t qf[16];
@@ -509,7 +518,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_fp4_kernel(const 
         pieces.tail = 1;
         pieces.tb = cu.b;
         pieces.th = cu.h;
-        pieces.over = warp_begin(warp) + cu.start + cu.nt - cta_tiles;
+        pieces.over = warp_begin(warp) + cu.start + cu.nt - cta_units;
       } else {
         pieces.head = 1;
         pieces.head_goes_on = goes_on;
@@ -517,8 +526,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_fp4_kernel(const 
         pieces.hh = cu.h;
       }
     }
-    if (seg_end < count) cu.next_item(a);
-    if (cu.b >= a.B) break;
+    if (seg_end == count) break;
+    cu.next_item(a);
+    r = cu.start;
   }
   cp_async_wait<0>();
   if (lane == 0) s_pieces[warp] = pieces;
@@ -658,9 +668,9 @@ __global__ void __launch_bounds__(kMergeThreads) merge_fp4_kernel(const __grid_c
 }
 
 // CTAs of the main kernel: what the SMs hold at once, fewer when even tables full of tokens would not
-// give every CTA kMinShare tiles.
+// give every CTA kMinShare units.
 int decode_fp4_ctas(int B, int Hkv, int max_blocks, int block_size, int num_sms) {
-  const int64_t most = (int64_t)B * Hkv * ((int64_t)max_blocks * (block_size / kTile));
+  const int64_t most = (int64_t)B * Hkv * ((int64_t)max_blocks * (block_size / kTile) + kItemUnits);
   const int64_t fill = (int64_t)num_sms * kCtasPerSm, need = (most + kMinShare - 1) / kMinShare;
   return (int)(need < fill ? (need > 0 ? need : 1) : fill);
 }
