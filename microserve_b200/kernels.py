@@ -382,7 +382,8 @@ def load_kv_fp4(k_cache: torch.Tensor, v_cache: torch.Tensor, k_scale: torch.Ten
         raise ValueError("load_kv_fp4: slot_mapping must be contiguous int64 [T]")
     _on_current_device("load_kv_fp4", k_cache, v_cache, k_scale, v_scale, slot_mapping)
     T = slot_mapping.shape[0]
-    k, v = k_cache.new_empty((2, T, Hkv, 128), dtype=torch.float16).unbind(0)
+    k = torch.empty(T, Hkv, 128, dtype=torch.float16, device=k_cache.device)
+    v = torch.empty_like(k)
     check(_lib.load().ms_load_kv_fp4(k_cache.data_ptr(), v_cache.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(),
                                      NB, BS, T, Hkv, 128, slot_mapping.data_ptr(), k.data_ptr(), v.data_ptr(),
                                      stream_ptr()), "ms_load_kv_fp4")
