@@ -409,12 +409,10 @@ def _fp4_query(what: str, query: torch.Tensor,
 
 
 def _int32(what: str, name: str, t: torch.Tensor, *shape: int) -> None:
-    if t.dtype is torch.int32 and t.is_contiguous() and t.dim() == len(shape):
-        for s, n in zip(shape, t.shape):
-            if s >= 0 and s != n:
-                break
-        else:
-            return
+    got = t.shape
+    if t.dtype is torch.int32 and t.is_contiguous() and (
+            got == shape or (shape[-1] < 0 and len(got) == len(shape) and got[:-1] == shape[:-1])):
+        return
     raise ValueError(f"{what}: {name} must be contiguous int32 of shape "
                      f"[{', '.join('*' if s < 0 else str(s) for s in shape)}]")
 
