@@ -216,9 +216,9 @@ struct PrefillArgs {
 // tensor core idles, count as kItemUnits more in front of its steps. (Without them the CTAs with the shortest items end
 // last: half as much time again for a ragged batch.)
 constexpr int kItemUnits = 4;
-// Units of a CTA at least. Two short tails on 300 to 700 tokens take 13.9 us with 4; 8 and 12 cost 3.7 and 7 us more: the
-// join costs less than a step or two.
-constexpr int kMinShare = 4;
+// Units of a CTA at least: the join costs less than a step or two. Two tails of 8 queries on 500 tokens take 13.3 us
+// with 3, 13.9 with 4, 12.8 with 2; one on 2400 takes 15.8 with 3 and 4, 16.6 with 2.
+constexpr int kMinShare = 3;
 constexpr int kPartRows = 2 * kRows;
 constexpr int kPartFloats = kPartRows * (kD + 2);  // O as [32 x 4 elements][row][4], then (reference, sum) per row
 
