@@ -150,6 +150,10 @@ class BlockManager:
         child.block_table.append(bid)
         return [(parent.block_table[full], bid, rest)]
 
+    def owns_a_block(self, seq: Sequence) -> bool:
+        """Whether deallocating `seq` frees a block (a fork may share all of its own)."""
+        return any(self.blocks[bid].ref_count == 1 for bid in seq.block_table)
+
     def deallocate(self, seq: Sequence) -> None:
         for bid in reversed(seq.block_table):
             self._unref(bid)

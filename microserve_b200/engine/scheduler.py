@@ -21,6 +21,11 @@ the reference and checks every round. The behaviour, as rules:
     the requester, nor already scheduled in this step, nor already preempted
     in it; its blocks are freed, it restarts from its prompt and goes to the
     head of the waiting queue.
+  * Forks (no counterpart in the reference) may share every block with others,
+    so that preempting one frees nothing. Among the victims one that owns a
+    block is taken first, and where none does, victims are taken until a block
+    is free. Without forks every sequence owns its last block, and one
+    victim is enough.
   * After the model ran, every scheduled sequence records the hashes of the
     blocks it filled and advances; a sequence whose scheduled tokens reached
     its end takes the sampled token (finishing on EOS, which is not appended,
@@ -151,17 +156,17 @@ class Scheduler:
             plan.take(seq, continued=False)
 
     def _reserve(self, seq: Sequence, plan: _StepPlan) -> bool:
-        """KV blocks and a token count for a running sequence, preempting one victim
-        if the blocks are short."""
+        """KV blocks and a token count for a running sequence, preempting victims
+        if the blocks are short (one, unless forks share its blocks)."""
         got = self.block_manager.allocate(seq, plan.budget)
-        if not got:
+        while not got:
             victim = self._pick_victim(seq, plan)
             if victim is None:
                 return False
             self.preempt(victim)
             plan.preempted.add(victim.seq_id)
             got = self.block_manager.allocate(seq, plan.budget)
-        if not got or (seq.gap != 1 and seq.num_scheduled_tokens == 0):
+        if seq.gap != 1 and seq.num_scheduled_tokens == 0:
             return False
         self._set_tokens(seq)
         return True
@@ -173,11 +178,14 @@ class Scheduler:
         seq.needs_sample = seq.num_computed_tokens + seq.num_scheduled_tokens == seq.num_tokens_with_spec
 
     def _pick_victim(self, requester: Sequence, plan: _StepPlan) -> Sequence | None:
+        newest = None
         for seq in reversed(self.running):
             if seq is requester or seq.seq_id in plan.continued or seq.seq_id in plan.preempted:
                 continue
-            return seq
-        return None
+            if self.block_manager.owns_a_block(seq):
+                return seq
+            newest = newest or seq
+        return newest
 
     def preempt(self, seq: Sequence) -> None:
         self.block_manager.deallocate(seq)
