@@ -45,7 +45,11 @@ class LLMEngine:
         child.num_prompt_tokens = seq.num_prompt_tokens
         copies = self.scheduler.fork(seq, child)
         if copies:
-            self.runner.copy_pages(copies)
+            try:
+                self.runner.copy_pages(copies)
+            except BaseException:  # the last page of `child` holds nothing: it must not run
+                self.scheduler.undo_fork(child)
+                raise
         return child
 
     def step(self) -> list[Sequence]:

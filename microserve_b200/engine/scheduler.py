@@ -98,6 +98,13 @@ class Scheduler:
         self.running.append(child)
         return copies
 
+    def undo_fork(self, child: Sequence) -> None:
+        """Take back a fork whose page copies could not be made: `child` leaves the running
+        sequences and gives up its blocks."""
+        self.running.remove(child)
+        self.block_manager.deallocate(child)
+        child.status, child.num_computed_tokens = SequenceStatus.WAITING, 0
+
     def is_idle(self) -> bool:
         return len(self.waiting) == 0 and len(self.running) == 0
 

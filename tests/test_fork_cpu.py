@@ -1,8 +1,10 @@
-"""Forks of running sequences on the host: preemption among sequences that share their blocks."""
+"""Forks of running sequences on the host: preemption among sequences that share their blocks, and forks whose
+page copies fail."""
 import random
 
 import pytest
 
+from microserve_b200.engine.llm import LLMEngine
 from microserve_b200.engine.scheduler import Scheduler
 from microserve_b200.engine.sequence import Sequence, SequenceStatus
 from tests.test_fp4_cpu import _fork, _running
@@ -76,3 +78,25 @@ def test_forked_runs_come_to_an_end(seed):
     assert sched.is_idle() and all(s.status == SequenceStatus.FINISHED for s in seqs)
     assert all(s.num_completion_tokens == s.max_tokens for s in seqs)
     assert not sched.block_manager.used_blocks
+
+
+class _NoCopies:
+    def copy_pages(self, pairs):
+        raise MemoryError("no room for the copies' arguments")
+
+
+def test_a_fork_whose_copies_fail_leaves_nothing_behind():
+    sched, seq = _prompts(6, 10)
+    eng = LLMEngine.__new__(LLMEngine)
+    eng.scheduler, eng.runner = sched, _NoCopies()
+    bm = sched.block_manager
+    cached = dict(bm.hash_to_block)
+    with pytest.raises(MemoryError):
+        eng.fork(seq)
+    assert list(sched.running) == [seq] and not sched.waiting
+    assert bm.free_blocks_nums == 3 and bm.hash_to_block == cached
+    _check_blocks(sched)
+    for _ in range(8):  # `seq` goes on alone
+        assert sched.schedule() == [seq]
+        sched.postprocess([seq], [3])
+        _check_blocks(sched)
