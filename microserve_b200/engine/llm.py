@@ -37,7 +37,9 @@ class LLMEngine:
         """A second sequence that continues from `seq`'s tokens and KV cache, between two steps (several
         samples of one prompt, a branch of a search). Full KV pages are shared; the partly filled
         last one is copied. The fork counts seq's prompt as its own and seq's completion so far as its
-        completion; its sampling parameters and max_tokens default to seq's. Raises ValueError if seq
+        completion; its sampling parameters and max_tokens default to seq's. `seq` may still be in its
+        prompt (chunked prefill): both then go through the rest of it. Under tensor parallelism every rank
+        calls it at the same step, as it does add() and step(). Raises ValueError if seq
         is not running or max_tokens is already reached, RuntimeError if max_num_seqs or the free KV
         blocks do not allow it."""
         child = Sequence(seq.token_ids, sampling_params=sampling_params or seq.sampling_params,

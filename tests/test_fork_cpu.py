@@ -1,8 +1,11 @@
-"""Forks of running sequences on the host: preemption among sequences that share their blocks, and forks whose
-page copies fail."""
+"""Forks of running sequences on the host: preemption among sequences that share their blocks, forks whose
+page copies fail, forks in the middle of a prompt, and forks on two tensor-parallel ranks."""
+import os
 import random
 
 import pytest
+import torch.distributed as dist
+import torch.multiprocessing as mp
 
 from microserve_b200.engine.llm import LLMEngine
 from microserve_b200.engine.scheduler import Scheduler
@@ -100,3 +103,86 @@ def test_a_fork_whose_copies_fail_leaves_nothing_behind():
         assert sched.schedule() == [seq]
         sched.postprocess([seq], [3])
         _check_blocks(sched)
+
+
+def test_fork_in_the_middle_of_a_prompt():
+    """22 tokens in chunks of 10: the fork shares the two full pages, gets a copy of the third and computes the rest
+    of the prompt into pages of its own."""
+    sched = Scheduler(16, 4, max_num_seqs=4, max_num_batched_tokens=10)
+    seq = Sequence(list(range(22)), max_tokens=3)
+    sched.add(seq)
+    sched.postprocess(sched.schedule(), [None])
+    assert seq.num_computed_tokens == 10
+    child, copies = _fork(sched, seq)
+    assert copies == [(seq.block_table[2], child.block_table[2], 2)] and child.block_table[:2] == seq.block_table[:2]
+    assert child.gap == seq.gap == 12 and child.num_completion_tokens == 0
+    while not sched.is_idle():
+        batch = sched.schedule()
+        sched.postprocess(batch, [7 if s.needs_sample else None for s in batch])
+        if child.block_table and seq.block_table:
+            assert not set(child.block_table[2:]) & set(seq.block_table[2:])
+        _check_blocks(sched)
+    assert seq.completion_token_ids == child.completion_token_ids == [7, 7, 7]
+    assert sched.block_manager.free_blocks_nums == 16
+
+
+class _Rank:
+    """A tensor-parallel rank's runner without a GPU: records the page copies, and every rank gets rank 0's tokens."""
+
+    def __init__(self):
+        self.copies = []
+
+    def copy_pages(self, pairs):
+        self.copies.append(pairs)
+
+    def execute(self, batch):
+        tokens = [random.randrange(50) if s.needs_sample else None for s in batch]  # every rank its own, but for:
+        dist.broadcast_object_list(tokens, src=0)
+        return tokens
+
+
+def _rank(rank, world, init_file, errq):
+    try:
+        dist.init_process_group("gloo", init_method=f"file://{init_file}", rank=rank, world_size=world)
+        eng = LLMEngine.__new__(LLMEngine)
+        eng.scheduler, eng.runner = Scheduler(20, 4, max_num_seqs=6, max_num_batched_tokens=12), _Rank()
+        r = random.Random(5)  # the program, the same on every rank
+        seqs = [eng.add(list(range(9 * i, 9 * i + 6 + 5 * i)), max_tokens=12) for i in range(3)]
+        trace = []
+        for step in range(200):
+            if eng.is_idle():
+                break
+            if step % 3 == 1 and eng.scheduler.running:
+                try:
+                    seqs.append(eng.fork(r.choice(list(eng.scheduler.running))))
+                except (RuntimeError, ValueError) as e:
+                    trace.append(str(e))
+            eng.step()
+            base = seqs[0].seq_id
+            trace.append([(s.seq_id - base, s.num_computed_tokens, list(s.block_table)) for s in eng.scheduler.running])
+        trace += [eng.runner.copies, [s.token_ids for s in seqs]]
+        assert eng.is_idle() and len(seqs) > 5 and eng.runner.copies
+        both = [None] * world
+        dist.all_gather_object(both, trace)
+        assert both[0] == both[1]
+        dist.barrier()
+        dist.destroy_process_group()
+    except Exception as ex:  # report to the parent
+        import traceback
+        errq.put(f"rank {rank}: {ex}\n{traceback.format_exc()}")
+        raise
+    os._exit(0)  # gloo's threads can abort a normal teardown
+
+
+def test_forks_on_two_ranks_take_the_same_blocks(tmp_path):
+    ctx = mp.get_context("spawn")
+    errq = ctx.Queue()
+    procs = [ctx.Process(target=_rank, args=(r, 2, str(tmp_path / "init"), errq)) for r in range(2)]
+    for p in procs:
+        p.start()
+    for p in procs:
+        p.join(180)
+    alive = [p for p in procs if p.is_alive()]
+    for p in alive:
+        p.kill()
+    assert not alive and all(p.exitcode == 0 for p in procs), errq.get() if not errq.empty() else "no answer"
