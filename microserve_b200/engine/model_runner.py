@@ -396,8 +396,9 @@ class ModelRunner:
             for m in self.model.modules():
                 if hasattr(m, "weight_fp8"):
                     gemm = max(gemm, lib.ms_fp8_gemm_workspace_size(bs, m.out_features, m.in_features))
-            decode = max(decode, kernels.decode_workspace_bytes(bs, hf.num_attention_heads // tp.tp_size(),
-                                                                self.num_kv_heads, max_blocks, self.block_size))
+            if self.config.kv_cache_dtype != "fp4_e2m1":  # the 4-bit cache's attention allocates its own per call
+                decode = max(decode, kernels.decode_workspace_bytes(bs, hf.num_attention_heads // tp.tp_size(),
+                                                                    self.num_kv_heads, max_blocks, self.block_size))
         kernels.workspace.reserve(gemm, self.device, "gemm")
         kernels.workspace.reserve(decode, self.device, "decode")
         kernels.workspace.reserve(lib.ms_argmax_workspace_size(max_bs), self.device, "argmax")
