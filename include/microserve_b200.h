@@ -225,7 +225,7 @@ int ms_load_kv_fp4(const void* k_cache, const void* v_cache, const void* k_scale
 
 /* ms_paged_decode_fp8 over the 4-bit cache: q [B, Hq, 128] fp16 with a token stride in
  * elements (heads contiguous), out [B, Hq, 128] fp16 (0 for seqlens == 0). Hq / Hkv <= 8,
- * softmax_scale > 0.
+ * 0 < softmax_scale <= 2e38.
  * A page outside the cache counts as masked, a length above max_blocks * block_size
  * is cut there (both recorded: device status 3). The workspace holds fp32 partials of the
  * call (ms_paged_decode_fp4_workspace_size bytes, 16-byte aligned, any contents); calls that
@@ -236,7 +236,7 @@ int ms_paged_decode_fp4(const void* q, int64_t q_token_stride, const void* k_cac
                         const int32_t* block_tables, void* out, int B, int Hq, int Hkv, int head_dim, int block_size,
                         int max_blocks, float softmax_scale, void* workspace, size_t workspace_bytes, void* stream);
 
-/* ms_paged_prefill_fp8 over the 4-bit cache, any Hq / Hkv <= 8, softmax_scale > 0: sequence s has queries
+/* ms_paged_prefill_fp8 over the 4-bit cache, any Hq / Hkv <= 8, the same scales: sequence s has queries
  * q[cu_q[s] .. cu_q[s+1]) at positions kv_lens[s] - q_len_s + i, each seeing the keys
  * up to its own position (none below position 0: output 0). Rows of out behind
  * cu_q[num_seqs] are not written, offsets outside [0, total_q] are cut. Workspace as for

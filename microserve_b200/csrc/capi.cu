@@ -69,8 +69,8 @@ int check_fp4_cache(const char* what, const void* k_cache, const void* v_cache, 
 // Query / output layout of the attentions over the 4-bit cache.
 int check_fp4_query(const char* what, const void* q, int64_t q_stride, const void* out, int Hq, int Hkv,
                     float softmax_scale) {
-  if (!(softmax_scale > 0.f) || softmax_scale > 3e38f)
-    return fail(MS_ERR_INVALID, "%s: softmax_scale must be a positive finite number", what);
+  if (!(softmax_scale > 0.f) || softmax_scale > 2e38f)  // times log2(e) it has to stay finite
+    return fail(MS_ERR_INVALID, "%s: softmax_scale must be positive and at most 2e38", what);
   if (Hq <= 0 || Hq % Hkv != 0 || Hq / Hkv > 8)
     return fail(MS_ERR_UNSUPPORTED, "%s: Hq=%d Hkv=%d unsupported (Hq a multiple of Hkv, at most 8 per kv head)", what,
                 Hq, Hkv);
