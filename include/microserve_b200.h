@@ -229,7 +229,8 @@ int ms_load_kv_fp4(const void* k_cache, const void* v_cache, const void* k_scale
  * A page outside the cache counts as masked, a length above max_blocks * block_size
  * is cut there (both recorded: device status 3). The workspace holds fp32 partials of the
  * call (ms_paged_decode_fp4_workspace_size bytes, 16-byte aligned, any contents); calls that
- * can overlap on the GPU need one each. */
+ * can overlap on the GPU need one each. Refused where B * Hkv * (max_blocks * block_size / 32)
+ * comes near 2^38 (a CTA counts its tiles in 32 bits). */
 size_t ms_paged_decode_fp4_workspace_size(int B, int Hq, int Hkv, int max_blocks, int block_size);
 int ms_paged_decode_fp4(const void* q, int64_t q_token_stride, const void* k_cache, const void* v_cache,
                         const void* k_scale, const void* v_scale, int64_t num_blocks, const int32_t* seqlens,

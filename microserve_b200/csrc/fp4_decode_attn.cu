@@ -707,6 +707,9 @@ cudaError_t launch_decode_fp4(const void* q, int64_t q_ts, const void* k_cache, 
   const int64_t cap = (int64_t)max_blocks * block_size;
   a.cap = (int)(cap < (1 << 30) ? cap : (1 << 30));
   a.scale_log2 = softmax_scale * kLog2e;
+  // a CTA counts its units in 32 bits, with room for one item more (2^30 on every SM's three CTAs: hours of work)
+  if ((double)B * Hkv * (a.cap / kTile + kItemUnits + 1) >= (double)num_sms * kCtasPerSm * (1 << 30))
+    return cudaErrorInvalidValue;
   const int ctas = decode_fp4_ctas(B, Hkv, max_blocks, block_size, num_sms);
   a.open_items = (int4*)workspace;
   a.ws = (float*)((int4*)workspace + ctas);
