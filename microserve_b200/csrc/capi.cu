@@ -342,7 +342,7 @@ int ms_load_kv_fp4(const void* k_cache, const void* v_cache, const void* k_scale
   if (!k || !v || !slots) return fail(MS_ERR_INVALID, "ms_load_kv_fp4: null pointer");
   if (!aligned16(k) || !aligned16(v)) return fail(MS_ERR_INVALID, "ms_load_kv_fp4: k and v must be 16-byte aligned");
   return check_cuda(ms::launch_load_kv_fp4(k_cache, v_cache, k_scale, v_scale, num_blocks, block_size, T, kv_heads,
-                                           slots, k, v, S(stream)),
+                                           slots, k, v, num_sms(), S(stream)),
                     "ms_load_kv_fp4");
 }
 

@@ -121,9 +121,9 @@ __global__ void __launch_bounds__(kThreads) load_kv_fp4_kernel(const __grid_cons
   }
 }
 
-// Two tokens a lane where that still gives 148 SMs several CTAs each, else one. Reading 32768 tokens x 8
+// Two tokens a lane where that still gives every SM several CTAs, else one. Reading 32768 tokens x 8
 // heads: 34.3 us with one, 31.8 with two, 36.0 with four.
-bool many_rows(int64_t T, int kv_heads) { return T * kv_heads >= 148 * 8 * kGroups; }
+bool many_rows(int64_t T, int kv_heads, int num_sms) { return T * kv_heads >= (int64_t)num_sms * 8 * kGroups; }
 template <int R>
 dim3 grid_for(int64_t T, int kv_heads) {
   return dim3((unsigned)((T + kGroups * R - 1) / (kGroups * R)), (unsigned)kv_heads);
@@ -165,11 +165,11 @@ cudaError_t launch_store_kv_fp4(const void* k, const void* v, int64_t k_ts, int6
 
 cudaError_t launch_load_kv_fp4(const void* k_cache, const void* v_cache, const void* k_scale, const void* v_scale,
                                int64_t num_blocks, int block_size, int64_t T, int kv_heads, const int64_t* slots,
-                               void* k, void* v, cudaStream_t stream) {
+                               void* k, void* v, int num_sms, cudaStream_t stream) {
   if (T == 0) return cudaSuccess;
   const KvFp4Args a = kv_args(k, v, T, kv_heads, slots, const_cast<void*>(k_cache), const_cast<void*>(v_cache),
                               const_cast<void*>(k_scale), const_cast<void*>(v_scale), num_blocks, block_size);
-  if (many_rows(T, kv_heads))
+  if (many_rows(T, kv_heads, num_sms))
     return launch_kernel(load_kv_fp4_kernel<2>, grid_for<2>(T, kv_heads), dim3(kThreads), 0, stream, a);
   return launch_kernel(load_kv_fp4_kernel<1>, grid_for<1>(T, kv_heads), dim3(kThreads), 0, stream, a);
 }

@@ -48,7 +48,7 @@ cudaError_t launch_store_kv_fp4(const void* k, const void* v, int64_t k_ts, int6
                                 cudaStream_t stream);
 cudaError_t launch_load_kv_fp4(const void* k_cache, const void* v_cache, const void* k_scale, const void* v_scale,
                                int64_t num_blocks, int block_size, int64_t T, int kv_heads, const int64_t* slots,
-                               void* k, void* v, cudaStream_t stream);
+                               void* k, void* v, int num_sms, cudaStream_t stream);
 size_t decode_fp4_workspace_bytes(int B, int Hq, int Hkv, int max_blocks, int block_size, int num_sms);
 cudaError_t launch_decode_fp4(const void* q, int64_t q_ts, const void* k_cache, const void* v_cache,
                               const void* k_scale, const void* v_scale, int64_t num_blocks, const int32_t* seqlens,
