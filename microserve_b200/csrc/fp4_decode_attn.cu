@@ -26,7 +26,8 @@
 //    8 tokens a thread needs of V are consecutive; neither changes a result.
 //  * Softmax in the exp2 domain, fp32 sums, with a lazy reference: weights are 2^(s - m)
 //    for a reference m that moves (and the sums are rescaled) only when a score exceeds it by
-//    5 or more, which after an item's first tile is rare. A weight enters the second
+//    5 or more, which after an item's first tile is rare (or is too far from zero for one rounding of
+//    its product with the scale: fp4_kv.cuh). A weight enters the second
 //    product as two f16 parts (hi + lo, scaled by 2^10: at most 2^15), so outputs keep
 //    fp32-level accuracy; with G <= 4 both parts share one MMA (columns 0-3 hi, 4-7 lo),
 //    with more heads it takes two.
@@ -320,8 +321,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_fp4_kernel(const 
     float acc[8][4];
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
-    float m_ref[2] = {-INFINITY, -INFINITY};  // columns 2c, 2c + 1: the reference less 10
+    float m_ref[2] = {-INFINITY, -INFINITY};  // columns 2c, 2c + 1: the reference, a score
+    float neg[2] = {INFINITY, INFINITY};      // 10 - m_ref scale_log2
     float l_run[2] = {0.f, 0.f};
+    bool far = false;  // some reference of the warp is a far score (fp4_kv.cuh): every tile takes the branch below
 
     for (; r < seg_end; ++r) {
       cp_async_wait<kStages - 1>();
@@ -356,31 +359,35 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_fp4_kernel(const 
       }
       // ---- softmax: exponents against the reference ------------------------------------
       float e[2][4];
-      auto exponents = [&] {
+      auto exponents = [&](bool is_far) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) e[t][j] = fmaf(s[t][j], a.scale_log2, -m_ref[j & 1]);
+          for (int j = 0; j < 4; ++j) {
+            e[t][j] = fmaf(s[t][j], a.scale_log2, neg[j & 1]);
+            if (is_far && far_score(m_ref[j & 1], a.scale_log2))
+              e[t][j] = fmaf(s[t][j] - m_ref[j & 1], a.scale_log2, kPScaleLog2);
+          }
           if (left < kTile) {
             if (tok_a + 4 * t >= left) e[t][0] = e[t][1] = -INFINITY;
             if (tok_a + 4 * t + 2 >= left) e[t][2] = e[t][3] = -INFINITY;
           }
         }
       };
-      exponents();
+      exponents(false);
       const float top = fmaxf(fmaxf(fmaxf(e[0][0], e[0][1]), fmaxf(e[0][2], e[0][3])),
                               fmaxf(fmaxf(e[1][0], e[1][1]), fmaxf(e[1][2], e[1][3])));
-      if (__any_sync(0xffffffffu, top > kPMaxLog2)) {  // move the reference to this tile's maximum
+      if (far || __any_sync(0xffffffffu, top > kPMaxLog2)) {  // move the reference to this tile's maximum
         float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
           if (tok_a + 4 * t < left) {
-            mx[0] = fmaxf(mx[0], s[t][0] * a.scale_log2);
-            mx[1] = fmaxf(mx[1], s[t][1] * a.scale_log2);
+            mx[0] = fmaxf(mx[0], s[t][0]);
+            mx[1] = fmaxf(mx[1], s[t][1]);
           }
           if (tok_a + 4 * t + 2 < left) {
-            mx[0] = fmaxf(mx[0], s[t][2] * a.scale_log2);
-            mx[1] = fmaxf(mx[1], s[t][3] * a.scale_log2);
+            mx[0] = fmaxf(mx[0], s[t][2]);
+            mx[1] = fmaxf(mx[1], s[t][3]);
           }
         }
         float al[2];
@@ -388,9 +395,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_fp4_kernel(const 
         for (int j = 0; j < 2; ++j) {
 #pragma unroll
           for (int o = 4; o < 32; o <<= 1) mx[j] = fmaxf(mx[j], __shfl_xor_sync(0xffffffffu, mx[j], o));
-          const float mn = fmaxf(m_ref[j], mx[j] - kPScaleLog2);
-          al[j] = m_ref[j] == -INFINITY ? 1.f : ex2(m_ref[j] - mn);  // nothing summed yet: nothing to rescale
+          const float mn = fmaxf(m_ref[j], mx[j]);
+          al[j] = m_ref[j] == -INFINITY ? 1.f : ex2((m_ref[j] - mn) * a.scale_log2);  // nothing summed yet: nothing to rescale
           m_ref[j] = mn;
+          neg[j] = fmaf(-mn, a.scale_log2, kPScaleLog2);
           l_run[j] *= al[j];
         }
 #pragma unroll
@@ -400,7 +408,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_fp4_kernel(const 
           acc[i][2] *= al[0];
           acc[i][3] *= al[1];
         }
-        exponents();
+        far = __any_sync(0xffffffffu, far_score(m_ref[0], a.scale_log2) || far_score(m_ref[1], a.scale_log2));
+        exponents(far);
       }
       uint32_t hi[2][2], lo[2][2];  // [MMA tile][rows 0-7, 8-15]
 #pragma unroll
@@ -544,8 +553,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_fp4_kernel(const 
   auto take = [&](const float* part) {
     const float* row = part + h * kRowFloats;
     const float m = row[kD], mn = fmaxf(M, m);
-    const float w0 = M == -INFINITY ? 1.f : ex2(M - mn);  // a sum without valid tokens is 0 (or NaN)
-    const float w1 = m == -INFINITY ? 1.f : ex2(m - mn);
+    const float w0 = M == -INFINITY ? 1.f : ex2((M - mn) * a.scale_log2);  // a sum without valid tokens is 0 (or NaN)
+    const float w1 = m == -INFINITY ? 1.f : ex2((m - mn) * a.scale_log2);
     M = mn;
     L = L * w0 + row[kD + 1] * w1;
     const float4 u0 = *reinterpret_cast<const float4*>(row + d0), u1 = *reinterpret_cast<const float4*>(row + d0 + 4);
@@ -618,7 +627,8 @@ __global__ void __launch_bounds__(kMergeThreads) merge_fp4_kernel(const __grid_c
   for (int i = 0; i < 8; ++i) o[i] = 0.f;
   auto take = [&](float m, float l, const float (&u)[8]) {
     const float mn = fmaxf(M, m);
-    const float w0 = M == -INFINITY ? 1.f : ex2(M - mn), w1 = m == -INFINITY ? 1.f : ex2(m - mn);
+    const float w0 = M == -INFINITY ? 1.f : ex2((M - mn) * a.scale_log2);
+    const float w1 = m == -INFINITY ? 1.f : ex2((m - mn) * a.scale_log2);
     M = mn;
     L = L * w0 + l * w1;
 #pragma unroll

@@ -79,6 +79,15 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
   return r;
 }
 
+// Softmax references are kept as scores r, and a weight is 2^((s - r) c + b) (c: the softmax scale times log2 e, b: a
+// constant). s c - (r c - b) is one fma a score, but r c is rounded by 2^-24 of itself, a factor that all weights
+// of a row share: harmless until it drives a weight out of f16's range. So where |r| c is above this, s - r is formed first.
+constexpr float kFarScore = 4194304.f;  // 2^22: the factor is below 2^(1/4)
+__device__ __forceinline__ bool far_score(float r, float c) {
+  const float x = fabsf(r) * c;
+  return x > kFarScore && x < INFINITY;  // (r infinite: nothing seen yet, or an infinite query)
+}
+
 // Scale byte of a group whose largest |x| has the fp16 bits `amax` (0..0x7FFF).
 // a / 6 is taken as a * h + a * l with h + l = 1/6 to 48 bits: exact where it is a rounding
 // boundary (5 bits), right to 2^-24 elsewhere.

@@ -31,7 +31,8 @@
 // m that moves, with a rescale of O in TMEM, only when a row's maximum exceeds it by 8 or
 // more. Weights are rounded to f16 for the second product (2^-11 relative, 2^-31 of the largest
 // where they are subnormal; the first rounding below fp32 in the kernel, K and V are exact), the
-// row sums take them unrounded.
+// row sums take them unrounded. Rows whose scores are too far from zero for that form (4 million and more) are done once
+// more at the end, from differences of scores (far_rows).
 //
 // V rows behind an item's last key and rows of bad pages are written as zeros, and a NaN group
 // of V as zeros too, because a zero weight does not hide a NaN from the product; where one was
@@ -198,6 +199,8 @@ __device__ __forceinline__ bool warp_wait(uint64_t* bar, uint32_t phase) {
 }
 
 struct PrefillArgs {
+  const __half* q;  // [T, Hq, D], token stride q_ts elements (read by TMA but for far scores)
+  int64_t q_ts;
   const uint8_t *kc, *vc, *ks, *vs;
   int64_t num_blocks;
   const int32_t* tables;  // [S, max_blocks]
@@ -205,7 +208,7 @@ struct PrefillArgs {
   const int32_t* kv_lens;
   __half* out;       // [T, Hq, D]
   int4* open_items;  // workspace: per CTA, the item that it leaves open: CTAs it goes on in, seq, block, kv head
-  float* ws;         // workspace: [CTAs][2] partials of kPartFloats
+  float* ws;         // workspace: [CTAs][2] partials of kPartFloats: O, and the reference (a score) and sum of each row
   int num_seqs, total_q, Hkv, G, tok, block_size, bs_log2, max_blocks;  // tok: query tokens of an item, 2 (128 / G)
   int inv_g;  // r / G = r * inv_g >> 16 for rows r of a tile
   int cap;  // tokens that a table row can hold
@@ -392,6 +395,81 @@ __device__ __forceinline__ int find_share(const PrefillArgs& a, Cursor& c, int64
   return c.j0 < c.j1 || c.next_item(a, count) ? count : 0;
 }
 
+// Outputs and partials once more where scores are so far from zero that the rounding of s c - (r c - b) would decide their
+// weights (far_score; from 2^27 on in the log2 domain weights would leave f16's range): the rows of the softmax warps that
+// met such a reference, in all items of the CTA, from differences of scores and in fp32. All warps, when the roles have
+// ended: a call inside the softmax loop cost 2 % there. A warp has a row, four keys at a time: some 100 cycles a key; rare.
+__device__ __noinline__ void far_rows(const PrefillArgs& a, Cursor c, int count, const int* far) {
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tpt = kRows / a.G;
+  auto values = [&](const uint8_t* codes, const uint8_t* scales, int64_t r, float (&x)[4]) {  // elements 4 lane ..
+    uint32_t o[4];
+    fp4x8_to_f16x2(*reinterpret_cast<const uint32_t*>(codes + r * kFp4RowBytes + (lane >> 1) * 4), o);
+    const uint32_t f = fp4_scale_h2(scales[r * kFp4ScaleBytes + (lane >> 2)]);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t w = h2_mul(lane & 1 ? o[2 + i] : o[i], f);
+      __half2 h;
+      memcpy(&h, &w, 4);
+      const float2 p = __half22float2(h);
+      x[2 * i] = p.x;
+      x[2 * i + 1] = p.y;
+    }
+  };
+  for (bool more = count > 0; more; more = c.next_item(a, count)) {
+    const int tok0 = c.b * a.tok, n_tok = min(a.tok, c.q.q_len - tok0), key_end = min(c.j1 * kKeys, c.keys);
+    for (int pr = warp; pr < kPartRows; pr += kThreads / 32) {
+      const int t = pr / kRows, row = pr % kRows, rt = row / a.G, tt = t * tpt + rt;
+      if (far[pr / 32] == 0 || rt >= tpt || tt >= n_tok) continue;
+      const int head = c.h * a.G + row - rt * a.G, tok = c.q.q_start + tok0 + tt;
+      const int end = min(min(c.q.prefix + tok0 + tt, c.q.kv_len - 1) + 1, key_end);
+      float q[4], m = -INFINITY, l = 0.f, o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) q[e] = __half2float(a.q[tok * a.q_ts + head * kD + 4 * lane + e]);
+      for (int k = c.j0 * kKeys; k < end; k += 4) {  // four keys lie in one page
+        const int pg = k / a.block_size;
+        const int64_t blk = pg < a.max_blocks ? a.tables[(int64_t)c.s * a.max_blocks + pg] : -1;
+        if (blk < 0 || blk >= a.num_blocks) continue;
+        const int64_t r = (blk * a.Hkv + c.h) * a.block_size + (k - pg * a.block_size);
+        float s[4], v[4][4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          float x[4];
+          values(a.kc, a.ks, r + u, x);
+          values(a.vc, a.vs, r + u, v[u]);
+          s[u] = q[0] * x[0] + q[1] * x[1] + q[2] * x[2] + q[3] * x[3];
+        }
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1)
+#pragma unroll
+          for (int u = 0; u < 4; ++u) s[u] += __shfl_xor_sync(0xffffffffu, s[u], d);
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          if (k + u >= end) break;
+          const float mn = fmaxf(m, s[u]);
+          const float w0 = m == -INFINITY ? 1.f : ex2((m - mn) * a.scale_log2);
+          // (a reference that is not far: as everywhere else, so that partials with the same one fit together)
+          const float w = ex2(far_score(mn, a.scale_log2)
+                                  ? fmaf(s[u] - mn, a.scale_log2, kPScaleLog2)
+                                  : fmaf(s[u], a.scale_log2, fmaf(-mn, a.scale_log2, kPScaleLog2)));
+          m = mn;
+          l = l * w0 + w;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) o[e] = o[e] * w0 + w * v[u][e];
+        }
+      }
+      if (c.j0 == 0 && c.j1 == c.steps) {
+        const float f = l == 0.f ? 0.f : 1.f / l;
+        *reinterpret_cast<uint2*>(a.out + ((int64_t)tok * a.Hkv * a.G + head) * kD + 4 * lane) =
+            make_uint2(pack_h2(o[0] * f, o[1] * f), pack_h2(o[2] * f, o[3] * f));
+      } else {
+        float* part = a.ws + ((int64_t)blockIdx.x * 2 + (c.j0 > 0 ? 0 : 1)) * kPartFloats;
+        *reinterpret_cast<float4*>(part + (lane * kPartRows + pr) * 4) = make_float4(o[0], o[1], o[2], o[3]);
+        if (lane == 0) *reinterpret_cast<float2*>(part + kPartRows * kD + pr * 2) = make_float2(m, l);
+      }
+    }
+  }
+}
+
 __global__ void __launch_bounds__(kThreads, 1)
     prefill_fp4_kernel(const __grid_constant__ CUtensorMap tmap_q, const __grid_constant__ PrefillArgs a) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
@@ -403,6 +481,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   __shared__ int64_t s_share;
   __shared__ int s_seen_nan;  // a V group with a NaN was decoded
   __shared__ int s_bad;       // a page outside the cache was met
+  __shared__ int s_far[8];    // per softmax warp: a row had a far score as its reference
   unsigned char* smem = smem_raw + ((1024 - (smem_u32(smem_raw) & 1023)) & 1023);
   unsigned char* s_q = smem;
   unsigned char* s_kv = smem + kQBytes;
@@ -423,6 +502,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       s_bad = 0;
       s_seen_nan = 0;
     }
+    if (lane < 8) s_far[lane] = 0;
   }
   if (warp == kMmaWarp + 1) {
     if (lane == 0) {
@@ -470,7 +550,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int low = lim;  // smallest limit of the warp: steps below it need no mask
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) low = min(low, __shfl_xor_sync(0xffffffffu, low, o));
-      float m = -INFINITY, l = 0.f;  // reference (log2 units, less kPScaleLog2) and sum
+      float m = -INFINITY, l = 0.f;  // reference (a score) and sum
       bool ok = true;
       for (int j = j0; j < j1; ++j, ++js) {
         ok = warp_wait(&s_full[t][js & 1], (js >> 1) & 1);
@@ -497,14 +577,15 @@ __global__ void __launch_bounds__(kThreads, 1)
             hide(v[c], seen);
           }
         }
-        const float mx = max32(v[1], max32(v[0], -INFINITY)) * a.scale_log2;
-        // ---- the reference moves when some row's maximum is far above it ---------------------
-        const bool far = mx - kPScaleLog2 > m + kMove || (m == -INFINITY && mx > -INFINITY);
+        const float mx = max32(v[1], max32(v[0], -INFINITY));
+        // ---- the reference moves when some row's maximum is far above it (or the first one) --------
+        const bool far = (mx - m) * a.scale_log2 > kMove;
         if (__any_sync(0xffffffffu, far)) {
-          const float mn = far ? mx - kPScaleLog2 : m;
-          const float al = m == -INFINITY ? 1.f : ex2(m - mn);
+          const float mn = far ? mx : m;
+          const float al = m == -INFINITY ? 1.f : ex2((m - mn) * a.scale_log2);
           m = mn;
           l *= al;
+          if (far_score(m, a.scale_log2)) s_far[warp] = 1;
           if (j > j0) {
             // S of this step was issued behind the product of step js - 2, so the phase of this barrier before
             // the awaited one is over
@@ -524,7 +605,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           }
         }
         // ---- weights, f16, over the scores ----------------------------------------------------
-        const float neg = m == -INFINITY ? 0.f : -m;
+        const float neg = m == -INFINITY ? 0.f : fmaf(-m, a.scale_log2, kPScaleLog2);
         const uint64_t sc2 = f32x2(a.scale_log2, a.scale_log2), neg2 = f32x2(neg, neg);
         uint64_t sum[2] = {0, 0};
 #pragma unroll
@@ -792,6 +873,10 @@ __global__ void __launch_bounds__(kThreads, 1)
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
   }
+  int far = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) far |= s_far[i];
+  if (far != 0) far_rows(a, s_first, count, s_far);
 }
 
 // Items that cross CTAs: block (i, y) joins 32 rows of the one that CTA i leaves open, if any, from its
@@ -820,7 +905,8 @@ __global__ void __launch_bounds__(kMergeThreads) merge_prefill_fp4_kernel(const 
     for (int i = 0; i < 4; ++i)
       u[i] = *reinterpret_cast<const float4*>(part + ((e0 / 4 + i) * kPartRows + row) * 4);
     const float mn = fmaxf(M, ml.x);
-    const float w0 = M == -INFINITY ? 1.f : ex2(M - mn), w1 = ml.x == -INFINITY ? 1.f : ex2(ml.x - mn);
+    const float w0 = M == -INFINITY ? 1.f : ex2((M - mn) * a.scale_log2);
+    const float w1 = ml.x == -INFINITY ? 1.f : ex2((ml.x - mn) * a.scale_log2);
     M = mn;
     L = L * w0 + ml.y * w1;
 #pragma unroll
@@ -862,6 +948,8 @@ cudaError_t launch_prefill_fp4(const void* q, int64_t q_ts, const void* k_cache,
                                int num_seqs, int total_q, int Hq, int Hkv, int block_size, int max_blocks,
                                float softmax_scale, void* workspace, int num_sms, cudaStream_t stream) {
   PrefillArgs a = {};
+  a.q = (const __half*)q;
+  a.q_ts = q_ts;
   a.kc = (const uint8_t*)k_cache;
   a.vc = (const uint8_t*)v_cache;
   a.ks = (const uint8_t*)k_scale;

@@ -1,7 +1,7 @@
 """The attentions over the 4-bit KV cache where scores climb, fall and jump along a sequence, so that the softmax
-reference moves and what was summed is rescaled.
+reference moves and what was summed is rescaled, and where scores are of the largest magnitudes.
 
-Only element 0 of the queries and keys is not zero, and it has few bits, so a score is exact in
+Only element 0 of the queries and keys is not zero in the first tests, and it has few bits, so a score is exact in
 fp32. With o the exact output and A = sum p |v|, an output may be off by its own rounding, 2^-11 |o| + 2^-25, and by
 A * (2^-12 + 2^-13): 2^-12 for the sums over up to 2^12 keys (2^-24 an addition), 2^-13 for the rest: a reference
 of up to 1200 in the log2 domain is rounded by 2^-24 * 1200 < 2^-13 / 1.4, and so is each of the two in a rescale, but what
@@ -102,3 +102,118 @@ def test_prefill_with_moving_references(shape, seqs, Hq, Hkv, BS):
     _within(got, o, a, max(kv), F.decode(c[1], c[3]).abs().max().item())
     for _ in range(5):
         assert torch.equal(kernels.paged_prefill_fp4(*args), got)
+
+
+# ------------------------------------------------------------------ the largest magnitudes
+def _filled(n, BS, k, seed):
+    """(block table, cache, fp64 values [n, 128]) of one sequence and kv head with keys k [n, 128]."""
+    bt, NB = _tables([n], BS, seed)
+    t = torch.arange(n)
+    g = torch.Generator().manual_seed(seed)
+    kk, vv = torch.zeros(NB, 1, BS, 128).half(), torch.randn(NB, 1, BS, 128, generator=g).half()
+    kk[bt[0].long()[t // BS], 0, t % BS] = k.half()
+    (kc, ks), (vc, vs) = F.encode(kk), F.encode(vv)
+    return bt, [kc, vc, ks, vs], F.gather(vc, vs, bt[0], n)[0]
+
+
+def _both(q, c, bt, n):
+    """(decode, prefill) outputs of queries [T, G, 128] on one sequence's n keys, each query on all of them."""
+    from microserve_b200 import kernels
+    T = q.shape[0]
+    many, lens = bt.expand(T, -1).contiguous().to(DEV), _i32([n] * T)
+    d = _dev(c)
+    return (kernels.paged_decode_fp4(q.to(DEV), *d, lens, many, SCALE).cpu().double(),
+            kernels.paged_prefill_fp4(q.to(DEV), *d, many, _i32(range(T + 1)), lens, SCALE).cpu().double())
+
+
+@pytest.mark.parametrize("n,G", [(1, 1), (64, 4), (65, 8), (700, 2), (2900, 7)])
+def test_equal_scores_of_any_magnitude(n, G):
+    """All keys alike, queries of 2^-4 to 2^15 of either sign: scores from 2^16 to 2^36 in the log2 domain and the
+    same ones negative. Every product and sum is exact, so every weight is the same: the mean of the values."""
+    bt, c, v = _filled(n, 64, torch.full((n, 128), 61440.0), 31)
+    e = torch.arange(-4, 16)
+    q = torch.cat([torch.exp2(e.double()), -torch.exp2(e.double())])[:, None, None].expand(-1, G, 128).half()
+    mean, a = v.mean(0), v.abs().mean(0)
+    decode, prefill = _both(q, c, bt, n)
+    _within(decode, mean.expand_as(decode), a)
+    _within(prefill, mean.expand_as(prefill), a, n, v.abs().max().item())
+
+
+@pytest.mark.parametrize("n", [2, 150, 2000])
+@pytest.mark.parametrize("sign", [1, -1])
+def test_one_key_wins_by_far(n, sign):
+    """Scores up to 2^35 in the log2 domain, one or two keys far above all others: their value, or the mean of two."""
+    g = torch.Generator().manual_seed(n)
+    for where in ({0}, {n - 1}, {n // 2}, {0, n - 1}, {n // 3, n // 2}):
+        # positive queries: the winners are the largest; negative ones: the least negative
+        k = (1000 * torch.rand(n, 128, generator=g) + 1) if sign > 0 else torch.full((n, 128), 60000.0)
+        for w in where:
+            k[w] = 60000.0 if sign > 0 else 30.0
+        bt, c, v = _filled(n, 64, k, 32)
+        q = torch.full((3, 4, 128), 60000.0 * sign).half()
+        q[1] = 7.0 * sign
+        q[2] = 900.0 * sign
+        want, a = v[sorted(where)].mean(0), v[sorted(where)].abs().mean(0)
+        decode, prefill = _both(q, c, bt, n)
+        _within(decode, want.expand_as(decode), a)
+        _within(prefill, want.expand_as(prefill), a, n, v.abs().max().item())
+
+
+def _levels(lens, BS, Hkv, seed):
+    """Keys of one element, of a few heights between 27648 and 38912, so that many are alike."""
+    g = torch.Generator().manual_seed(seed)
+    bt, NB = _tables(lens, BS, seed)
+    k = torch.zeros(NB, Hkv, BS, 128, dtype=torch.float16)
+    k[..., 0] = (28000 + 10000 * torch.rand(NB, Hkv, BS, generator=g)).half()
+    v = torch.randn(NB, Hkv, BS, 128, generator=g).half()
+    (kc, ks), (vc, vs) = F.encode(k), F.encode(v)
+    return bt, [kc, vc, ks, vs]
+
+
+def _expected(q, c, table, n, bad):
+    """attend() of the oracle, with the pages `bad` masked."""
+    Q, Hq, _ = q.shape
+    BS, G = c[0].shape[2], Hq // c[0].shape[1]
+    good = table.clone()
+    good[good < 0] = 0
+    k, v = F.gather(c[0], c[2], good, n), F.gather(c[1], c[3], good, n)
+    t = torch.arange(n)
+    seen = (t[None, :] <= (n - Q + torch.arange(Q))[:, None]) & ~torch.isin(t // BS, torch.tensor(bad))[None, :]
+    o, a = torch.zeros(Q, Hq, 128, dtype=torch.float64), torch.zeros(Q, Hq, 128, dtype=torch.float64)
+    for h in range(Hq):
+        s = (q[:, h].double() @ k[h // G].t() * SCALE).masked_fill(~seen, float("-inf"))
+        p = torch.softmax(s, -1).nan_to_num(0.0)  # a row that sees nothing
+        o[:, h], a[:, h] = p @ v[h // G], p @ v[h // G].abs()
+    return o, a
+
+
+@pytest.mark.parametrize("Hq,Hkv,BS", [(16, 2, 64), (3, 1, 128), (8, 8, 64), (24, 4, 192)])
+@pytest.mark.parametrize("masked", [False, True])
+def test_far_and_near_rows_side_by_side(Hq, Hkv, BS, masked):
+    """Rows with scores of 2^26 and more beside rows with scores of about 60, in items inside and across CTAs, with
+    strided queries and, `masked`, pages outside the cache; far rows weigh the keys at the top level alike."""
+    from microserve_b200 import _lib, kernels
+    values = (2.0 ** 15, 2.0 ** -6, -(2.0 ** 15), 2.0 ** -7, 0.0, 2.0 ** 14, -(2.0 ** -6))
+    seqs = [(70, 500), (3, 0), (0, 40), (129, 700), (1, 1800)]
+    kv, cu = [q + p for q, p in seqs], [0]
+    for n, _ in seqs:
+        cu.append(cu[-1] + n)
+    bt, c = _levels(kv, BS, Hkv, Hq)
+    bad = {0: [1], 3: [0, 3], 4: [5]} if masked else {}
+    for s, pages in bad.items():
+        bt[s, pages] = torch.tensor([[-1, 1 << 30][i % 2] for i in range(len(pages))], dtype=torch.int32)
+    tables = torch.where(bt >= c[0].shape[0], -1, bt)
+    q = _one_element(cu[-1], Hq, values)
+    wide = torch.full((cu[-1], Hq + 1, 128), 5.0, dtype=torch.float16)
+    wide[:, :Hq] = q
+    vmax = F.decode(c[1], c[3]).abs().max().item()
+    want = [_expected(q[cu[s]:cu[s + 1]], c, tables[s], kv[s], bad.get(s, [])) for s in range(len(seqs)) if seqs[s][0]]
+    o, a = torch.cat([x[0] for x in want]), torch.cat([x[1] for x in want])
+    got = kernels.paged_prefill_fp4(wide.to(DEV)[:, :Hq], *_dev(c), bt.to(DEV), _i32(cu), _i32(kv), SCALE)
+    _within(got, o, a, max(kv), vmax)
+    # each sequence's last query, as a decode step
+    last = [cu[s + 1] - 1 for s in range(len(seqs)) if seqs[s][0]]
+    rows = [s for s in range(len(seqs)) if seqs[s][0]]
+    got = kernels.paged_decode_fp4(wide[last].to(DEV)[:, :Hq], *_dev(c), _i32([kv[s] for s in rows]), bt[rows].to(DEV), SCALE)
+    _within(got, o[last], a[last])
+    assert _lib.device_status() == (3 if masked else 0)
