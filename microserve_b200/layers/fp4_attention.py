@@ -22,4 +22,5 @@ def fp4_varlen_chunk_prefill_attention(query: torch.Tensor, k_cache: torch.Tenso
     """Causal attention of every sequence of a chunked-prefill batch: sequence s has queries
     cu_seqlens_q[s]:cu_seqlens_q[s+1] and kv_lens[s] cached tokens (this chunk's included)."""
     return kernels.paged_prefill_fp4(query, k_cache, v_cache, k_scale_cache, v_scale_cache,
-                                     block_tables.contiguous(), cu_seqlens_q, kv_lens, softmax_scale, out=out)
+                                     block_tables.contiguous(), cu_seqlens_q.contiguous(), kv_lens.contiguous(),
+                                     softmax_scale, out=out)
