@@ -322,10 +322,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_fp4_kernel(const 
 #pragma unroll
     for (int i = 0; i < 8; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
     float m_ref[2] = {-INFINITY, -INFINITY};  // columns 2c, 2c + 1: the reference, a score
-    float neg[2] = {INFINITY, INFINITY};      // 10 - m_ref scale_log2
+    // 10 - m_ref scale_log2; infinite where the reference is a far score (fp4_kv.cuh), so that tiles with keys take the
+    // branch below, which forms differences
+    float neg[2] = {INFINITY, INFINITY};
     float l_run[2] = {0.f, 0.f};
-    bool far = false;  // some reference of the warp is a far score (fp4_kv.cuh): every tile takes the branch below
-
     for (; r < seg_end; ++r) {
       cp_async_wait<kStages - 1>();
       __syncwarp();
@@ -359,13 +359,13 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_fp4_kernel(const 
       }
       // ---- softmax: exponents against the reference ------------------------------------
       float e[2][4];
-      auto exponents = [&](bool is_far) {
+      auto exponents = [&](bool differences) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
             e[t][j] = fmaf(s[t][j], a.scale_log2, neg[j & 1]);
-            if (is_far && far_score(m_ref[j & 1], a.scale_log2))
+            if (differences && neg[j & 1] == INFINITY)
               e[t][j] = fmaf(s[t][j] - m_ref[j & 1], a.scale_log2, kPScaleLog2);
           }
           if (left < kTile) {
@@ -377,7 +377,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_fp4_kernel(const 
       exponents(false);
       const float top = fmaxf(fmaxf(fmaxf(e[0][0], e[0][1]), fmaxf(e[0][2], e[0][3])),
                               fmaxf(fmaxf(e[1][0], e[1][1]), fmaxf(e[1][2], e[1][3])));
-      if (far || __any_sync(0xffffffffu, top > kPMaxLog2)) {  // move the reference to this tile's maximum
+      if (__any_sync(0xffffffffu, top > kPMaxLog2)) {  // move the reference to this tile's maximum
         float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -398,7 +398,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_fp4_kernel(const 
           const float mn = fmaxf(m_ref[j], mx[j]);
           al[j] = m_ref[j] == -INFINITY ? 1.f : ex2((m_ref[j] - mn) * a.scale_log2);  // nothing summed yet: nothing to rescale
           m_ref[j] = mn;
-          neg[j] = fmaf(-mn, a.scale_log2, kPScaleLog2);
+          neg[j] = far_score(mn, a.scale_log2) ? INFINITY : fmaf(-mn, a.scale_log2, kPScaleLog2);
           l_run[j] *= al[j];
         }
 #pragma unroll
@@ -408,8 +408,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_fp4_kernel(const 
           acc[i][2] *= al[0];
           acc[i][3] *= al[1];
         }
-        far = __any_sync(0xffffffffu, far_score(m_ref[0], a.scale_log2) || far_score(m_ref[1], a.scale_log2));
-        exponents(far);
+        exponents(true);
       }
       uint32_t hi[2][2], lo[2][2];  // [MMA tile][rows 0-7, 8-15]
 #pragma unroll
