@@ -8,7 +8,7 @@
 // keys that both tiles read. The steps of all items (sequence, block of tokens, kv head) form
 // one list that is dealt evenly to one CTA per SM, whatever the lengths are; an item that
 // crosses CTAs leaves fp32 partials (O, reference, sum) in the workspace, joined by a second kernel.
-// 2048 queries behind 30720 tokens (32 / 8 heads) take 1010 us, 1055 TFLOP/s of visible pairs.
+// 2048 queries behind 30720 tokens (32 / 8 heads) take 1001 us, 1064 TFLOP/s of visible pairs.
 // The roles below walk a CTA's items on their own, so decoding runs ahead into the next one.
 //   warps 0-3, 4-7   softmax of tile 0 / 1: a thread owns a row. It reads its 64 scores of a
 //                    step from TMEM, writes the weights over them as f16, and keeps the row's
@@ -398,8 +398,10 @@ __device__ __forceinline__ int find_share(const PrefillArgs& a, Cursor& c, int64
 // Outputs and partials once more where scores are so far from zero that the rounding of s c - (r c - b) would decide their
 // weights (far_score; from 2^27 on in the log2 domain weights would leave f16's range): the rows of the softmax warps that
 // met such a reference, in all items of the CTA, from differences of scores and in fp32. All warps, when the roles have
-// ended: a call inside the softmax loop cost 2 % there. A warp has a row, four keys at a time: some 100 cycles a key; rare.
-__device__ __noinline__ void far_rows(const PrefillArgs& a, Cursor c, int count, const int* far) {
+// ended: a call inside the softmax loop cost 2 % there (and the cursor passed by value 1.5 % of a ragged batch). A warp has
+// a row, four keys at a time. Rare, so simple: 2048 queries on 32768 keys (32 / 8 heads), every row far, take 290 ms.
+__device__ __noinline__ void far_rows(const PrefillArgs& a, const Cursor* first, int count, const int* far) {
+  Cursor c = *first;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, tpt = kRows / a.G;
   auto values = [&](const uint8_t* codes, const uint8_t* scales, int64_t r, float (&x)[4]) {  // elements 4 lane ..
     uint32_t o[4];
@@ -876,7 +878,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   int far = 0;
 #pragma unroll
   for (int i = 0; i < 8; ++i) far |= s_far[i];
-  if (far != 0) far_rows(a, s_first, count, s_far);
+  if (far != 0) far_rows(a, &s_first, s_count, s_far);
 }
 
 // Items that cross CTAs: block (i, y) joins 32 rows of the one that CTA i leaves open, if any, from its
