@@ -66,8 +66,8 @@ int ms_set_pair_tiles(int enable);
 /* Reads and clears the device status word of the current device. Kernels
  * that wait on barriers give up after a bounded time, record a non-zero code
  * there (1 = tensor-core pipeline timeout, 2 = peer timeout) and return. The
- * 4-bit cache's kernels and ms_copy_pages skip a slot, page or length outside
- * the cache and record 3.
+ * 4-bit cache's kernels and ms_copy_pages skip a slot or page outside the cache,
+ * the attentions cut a length past a table's end, and record 3.
  * Synchronises `stream`. */
 int ms_get_device_status(int* status, void* stream);
 
@@ -205,8 +205,9 @@ int ms_varlen_prefill(const void* q, const void* k, const void* v, const int32_t
  *   k_cache, v_cache [num_blocks, kv_heads, block_size, 64] uint8
  *   k_scale, v_scale [num_blocks, kv_heads, block_size, 8] uint8
  * head_dim == 128, block_size % 64 == 0, num_blocks * block_size < 2^31, all four
- * 16-byte aligned. Slots, pages and lengths outside the cache are skipped on the GPU
- * and recorded (device status 3). */
+ * 16-byte aligned. Slots, pages and lengths outside the cache are skipped or cut on the
+ * GPU and recorded (device status 3); a negative slot is skipped and a negative length
+ * counts as 0 without a record. */
 
 /* Quantise-on-write of k, v [T, kv_heads, 128] fp16 at slots [T] int64 (block *
  * block_size + offset; negative = skip). Strides in elements (multiples of 8, the
@@ -240,8 +241,9 @@ int ms_paged_decode_fp4(const void* q, int64_t q_token_stride, const void* k_cac
 /* ms_paged_prefill_fp8 over the 4-bit cache, any Hq / Hkv <= 8, the same scales: sequence s has queries
  * q[cu_q[s] .. cu_q[s+1]) at positions kv_lens[s] - q_len_s + i, each seeing the keys
  * up to its own position (none below position 0: output 0). Rows of out behind
- * cu_q[num_seqs] are not written, offsets outside [0, total_q] are cut. Workspace as for
- * ms_paged_decode_fp4. Refused where (total_q * Hq / Hkv / 256 + num_seqs) * Hkv *
+ * cu_q[num_seqs] are not written, offsets outside [0, total_q] are cut (no record). Workspace as for
+ * ms_paged_decode_fp4: two partials of 133 KB for each CTA, of which there is one per SM at most
+ * (39 MB on 148 SMs), whether or not items cross CTAs. Refused where (total_q * Hq / Hkv / 256 + num_seqs) * Hkv *
  * (max_blocks * block_size / 64) comes near 2^31 (steps are counted in 32 bits). */
 size_t ms_paged_prefill_fp4_workspace_size(int num_seqs, int64_t total_q, int Hq, int Hkv, int max_blocks,
                                            int block_size);
@@ -258,7 +260,8 @@ int ms_paged_prefill_fp4(const void* q, int64_t q_token_stride, const void* k_ca
  * head_dim, scale_row_bytes = kv_heads * 4; 4-bit cache outer = kv_heads, 64 and 8. Plane
  * p's pages start at cache + p * cache_plane_stride bytes. A page may be the source of
  * any number of pairs but the destination of one, and no page both; pairs outside
- * [0, num_pages) are skipped (device status 3). No reference counterpart. */
+ * [0, num_pages) are skipped (device status 3), token counts outside [0, block_size] are
+ * cut (no record). No reference counterpart. */
 int ms_copy_pages(void* cache, int64_t cache_plane_stride, int row_bytes, void* scale, int64_t scale_plane_stride,
                   int scale_row_bytes, int planes, int outer, int block_size, int64_t num_pages, const int32_t* src,
                   const int32_t* dst, const int32_t* tokens, int n, void* stream);

@@ -2,12 +2,12 @@
 // per sequence:
 //   o[b, hq] = softmax_t(q[b, hq] . k[t] * scale) . v[t],  t < seqlens[b];  0 for no token.
 //
-// Bound by the cache's bytes (144 per token and kv head) and, close behind, by the
-// instructions that turn 4-bit codes into f16 operands, so both are kept even and few.
-// 241 MB of cache (256 sequences of 128 to 1536 tokens, 32 / 8 heads) take 58 us, 0.64 of the copy bandwidth:
+// Its floor is the cache's bytes (144 per token and kv head); what binds it now is waiting inside a warp's one chain per
+// tile (decode K, scores, softmax, decode V, product), nothing of the next tile being mixed in.
+// 241 MB of cache (256 sequences of 128 to 1536 tokens, 32 / 8 heads) take 58.7 us, 0.63 of the copy bandwidth:
 // 4.5 us to the first tile (scan, page look-up, copy: three memory latencies), 46 to 50 for an SM's tiles (its
-// copies alone 44, its arithmetic alone 54 with the overheads: 640 instructions a tile and warp at 0.54 a cycle and
-// scheduler), 3 for the join, 2.5 for the second kernel.
+// copies alone 44, its arithmetic alone 54 with the overheads, where the issue of 640 instructions a tile and warp would
+// take 30: a scheduler issues 0.54 of the time), 3 for the join, 2.5 for the second kernel.
 //  * The work is one flat list of 32-token tiles over (sequence, kv head, tile). The grid
 //    fills the SMs once; every CTA takes an equal contiguous share of the list, an item's own
 //    cost counted like a tile (found by a scan of seqlens), and every warp a quarter of that,
