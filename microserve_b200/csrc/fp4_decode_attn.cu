@@ -326,6 +326,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) decode_fp4_kernel(const 
     // branch below, which forms differences
     float neg[2] = {INFINITY, INFINITY};
     float l_run[2] = {0.f, 0.f};
+
     for (; r < seg_end; ++r) {
       cp_async_wait<kStages - 1>();
       __syncwarp();

@@ -84,8 +84,7 @@ __device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
 // of a row share: harmless until it drives a weight out of f16's range. So where |r| c is above this, s - r is formed first.
 constexpr float kFarScore = 4194304.f;  // 2^22: the factor is below 2^(1/4)
 __device__ __forceinline__ bool far_score(float r, float c) {
-  const float x = fabsf(r) * c;
-  return x > kFarScore && x < INFINITY;  // (r infinite: nothing seen yet, or an infinite query)
+  return fabsf(r) * c > kFarScore && fabsf(r) < INFINITY;  // (r infinite: nothing seen yet, or an infinite query)
 }
 
 // Scale byte of a group whose largest |x| has the fp16 bits `amax` (0..0x7FFF).

@@ -217,3 +217,19 @@ def test_far_and_near_rows_side_by_side(Hq, Hkv, BS, masked):
     got = kernels.paged_decode_fp4(wide[last].to(DEV)[:, :Hq], *_dev(c), _i32([kv[s] for s in rows]), bt[rows].to(DEV), SCALE)
     _within(got, o[last], a[last])
     assert _lib.device_status() == (3 if masked else 0)
+
+
+@pytest.mark.parametrize("scale", [1e-30, 1e-6, 1e8, 1e30, 2e38])
+def test_softmax_scales_of_any_size(scale):
+    """Scales so small that every key weighs the same and so large that scores times the scale pass fp32: the mean of
+    all values, and of those of the largest score."""
+    from microserve_b200 import kernels
+    n, Hq, T = 900, 8, 40
+    bt, c = _levels([n], 64, 2, 5)
+    q = _one_element(T, Hq, (1.0, -1.0, 0.0, 2.0 ** 15, -64.0))
+    o, a = F.attend(q, *c, bt[0], n, scale)
+    vmax = F.decode(c[1], c[3]).abs().max().item()
+    d = _dev(c)
+    _within(kernels.paged_prefill_fp4(q.to(DEV), *d, bt.to(DEV), _i32([0, T]), _i32([n]), scale), o, a, n, vmax)
+    got = kernels.paged_decode_fp4(q[-1:].to(DEV), *d, _i32([n]), bt.to(DEV), scale)
+    _within(got, o[-1:], a[-1:])
