@@ -238,13 +238,14 @@ int ms_paged_decode_fp4(const void* q, int64_t q_token_stride, const void* k_cac
                         const int32_t* block_tables, void* out, int B, int Hq, int Hkv, int head_dim, int block_size,
                         int max_blocks, float softmax_scale, void* workspace, size_t workspace_bytes, void* stream);
 
-/* ms_paged_prefill_fp8 over the 4-bit cache, any Hq / Hkv <= 8, the same scales: sequence s has queries
- * q[cu_q[s] .. cu_q[s+1]) at positions kv_lens[s] - q_len_s + i, each seeing the keys
- * up to its own position (none below position 0: output 0). Rows of out behind
- * cu_q[num_seqs] are not written, offsets outside [0, total_q] are cut (no record). Workspace as for
- * ms_paged_decode_fp4: two partials of 133 KB for each CTA, of which there is one per SM at most
- * (39 MB on 148 SMs), whether or not items cross CTAs. Refused where (total_q * Hq / Hkv / 256 + num_seqs) * Hkv *
- * (max_blocks * block_size / 64) comes near 2^31 (steps are counted in 32 bits). */
+/* ms_paged_prefill_fp8 over the 4-bit cache, any Hq / Hkv <= 8, the same scales: sequence s
+ * has queries q[cu_q[s] .. cu_q[s+1]) at positions kv_lens[s] - q_len_s + i, each seeing the
+ * keys up to its own position (none below position 0: output 0). Rows of out behind
+ * cu_q[num_seqs] are not written, offsets outside [0, total_q] are cut (no record). out must
+ * not overlap q. Workspace as for ms_paged_decode_fp4: two partials of 133 KB for each CTA, of
+ * which there is one per SM at most (39 MB on 148 SMs), whether or not items cross CTAs.
+ * Refused where (total_q * Hq / Hkv / 256 + num_seqs) * Hkv * (max_blocks * block_size / 64)
+ * comes near 2^31 (steps are counted in 32 bits). */
 size_t ms_paged_prefill_fp4_workspace_size(int num_seqs, int64_t total_q, int Hq, int Hkv, int max_blocks,
                                            int block_size);
 int ms_paged_prefill_fp4(const void* q, int64_t q_token_stride, const void* k_cache, const void* v_cache,

@@ -455,7 +455,7 @@ def paged_prefill_fp4(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
                       softmax_scale: float, out: torch.Tensor | None = None) -> torch.Tensor:
     """Causal attention of new tokens query [T, Hq, 128] fp16 (any token stride) over prefix + themselves
     in the 4-bit cache, every sequence in one launch. Rows behind cu_q[-1] are not written (pass `out`
-    to keep theirs). ms_paged_prefill_fp4."""
+    to keep theirs; where it shares memory with query, the query is copied). ms_paged_prefill_fp4."""
     T, Hq, D = query.shape
     NB, Hkv, BS = _fp4_cache("paged_prefill_fp4", k_cache, v_cache, k_scale, v_scale, D)
     num_seqs = kv_lens.shape[0]
@@ -463,6 +463,10 @@ def paged_prefill_fp4(query: torch.Tensor, k_cache: torch.Tensor, v_cache: torch
     _int32("paged_prefill_fp4", "cu_q", cu_q, num_seqs + 1)
     _int32("paged_prefill_fp4", "block_tables", block_tables, num_seqs, -1)
     query, q_stride, o = _fp4_query("paged_prefill_fp4", query, out)
+    if out is not None and T > 0:  # a CTA may read rows of the query after others have written theirs of the output
+        q_at, o_at, row = query.data_ptr(), o.data_ptr(), 2 * Hq * D
+        if q_at < o_at + T * row and o_at < q_at + (T - 1) * 2 * q_stride + row:
+            query, q_stride = query.clone(memory_format=torch.contiguous_format), Hq * D
     _on_current_device("paged_prefill_fp4", query, k_cache, v_cache, k_scale, v_scale, block_tables, cu_q, kv_lens, o)
     max_blocks = block_tables.shape[1]
     # its own for every call, as in paged_decode_fp4

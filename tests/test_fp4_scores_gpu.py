@@ -233,3 +233,24 @@ def test_softmax_scales_of_any_size(scale):
     _within(kernels.paged_prefill_fp4(q.to(DEV), *d, bt.to(DEV), _i32([0, T]), _i32([n]), scale), o, a, n, vmax)
     got = kernels.paged_decode_fp4(q[-1:].to(DEV), *d, _i32([n]), bt.to(DEV), scale)
     _within(got, o[-1:], a[-1:])
+
+
+def test_outputs_over_the_queries():
+    """`out` is the query itself, or shares its memory: rows with far scores and without, items inside CTAs and across."""
+    from microserve_b200 import kernels
+    Hq, Hkv, seqs = 32, 8, [(64, 64)] * 60 + [(3, 1500)]
+    kv, T = [a + b for a, b in seqs], sum(a for a, _ in seqs)
+    bt, c = _levels(kv, 64, Hkv, 6)
+    q = _one_element(T, Hq, (2.0 ** 15, 2.0 ** -6, -(2.0 ** 15), 0.0, 2.0 ** -7))
+    cu = [64 * i for i in range(61)] + [T]
+    args = (*_dev(c), bt.to(DEV), _i32(cu), _i32(kv), SCALE)
+    want = kernels.paged_prefill_fp4(q.to(DEV), *args)
+    same = q.to(DEV)
+    assert kernels.paged_prefill_fp4(same, *args, out=same) is same and torch.equal(same, want)
+    shared = torch.zeros(T + 3, Hq, 128, dtype=torch.float16, device=DEV)
+    shared[3:] = q.to(DEV)
+    got = kernels.paged_prefill_fp4(shared[3:], *args, out=shared[:T])
+    assert torch.equal(got, want)
+    last, args = q[-1:].to(DEV), (*_dev(c), _i32(kv[-1:]), bt[-1:].to(DEV), SCALE)
+    want = kernels.paged_decode_fp4(last, *args)
+    assert torch.equal(kernels.paged_decode_fp4(last, *args, out=last), want)
